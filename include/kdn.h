@@ -347,6 +347,64 @@ int kdn_varlen_causal_attention(const void* q, const void* k_cache, const void* 
                                 int64_t max_seqlen, void* out, void* stream);
 
 /*
+ * Losses over vocabulary logits (no reference entry points; the reference trains with torch's losses, and upcycles a
+ * teacher's layers in pipeline/transmute.py).  logits [n, V] (dtype KDN_DTYPE_F32 or KDN_DTYPE_BF16), rows ld elements
+ * apart (ld >= V, any ld and any element-aligned start; rows of one 16-byte phase move by vectors).  x = logits /
+ * temperature, log q = x - log sum e^x; sums and statistics are fp32.  dlogits (same dtype, rows ld_d apart; must not
+ * overlap logits) is the gradient of the loss, rounded once; NULL: no gradient is formed.  logits equal to -inf have
+ * probability zero; a row of nothing else, or with a NaN or +inf, gives NaN.
+ *
+ * A row whose label is ignore_index counts for nothing: its logits are not read, its outputs and its gradient row are
+ * zero.  A label outside [0, V) is treated the same way and recorded for kdn_device_error (code 1).  weights [n] fp32
+ * multiply each row's loss (a row of weight zero adds nothing to the loss or the gradient, whatever it holds); NULL
+ * means the mean over the rows that count.  Nothing here depends on an order of atomics: equal calls give equal bits.
+ *
+ *   kdn_token_logprobs: logps[t] = log q[t, labels[t]]; row_stats (may be NULL) [n, 2] fp32: a row's largest logit m
+ *     and sum_j e^((z_j - m) / T), which kdn_token_logprobs_backward reads.
+ *   kdn_token_logprobs_backward: dlogits[t, j] = dlogps[t] (1[j = label] - q[t, j]) / T (zero where dlogps[t] is).
+ *   kdn_policy_loss: with r = e^(logp - old_logps), g = ref_logps - logp and H the entropy of q,
+ *     loss = sum_t w_t (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^g - 1 - g) - entropy_coef H),
+ *     A = advantages; ref_logps may be NULL when kl_coef is 0; entropy [n] may be NULL.  loss: one fp32.
+ *   kdn_preference_loss: sequence s holds rows [cu_seqlens[s], cu_seqlens[s + 1]) (device int64 [2 pairs + 1]; rows
+ *     outside get a zero gradient); pair p prefers sequence 2 p to 2 p + 1.  log_ratios[s] = sum over its counting rows
+ *     of logp - ref_logps (NULL: 0), divided by their number with length_normalised; h = beta (log_ratios[2 p] -
+ *     log_ratios[2 p + 1]); loss = mean over pairs of -(1 - label_smoothing) log sigmoid(h) - label_smoothing
+ *     log sigmoid(-h).  A sequence of no counting row has log ratio 0.
+ *   kdn_distillation_loss: the teacher's `top` largest logits of each row and their ids [n, top] (ids in index_dtype;
+ *     negative ids are padding, and a row whose FIRST id is negative counts for nothing; an id >= V is skipped and
+ *     recorded, code 1; an id given twice counts twice).  teacher_lse NULL: p = softmax of the row's entries / T; else
+ *     p = e^(teacher / T - teacher_lse[t]) (log-sum-exp of the teacher's whole row / T) and what is left of the
+ *     teacher's mass, 1 - sum p, is compared with the student's mass outside the ids as one more class.
+ *     divergence[t] = KL(p || q), loss = T^2 sum_t w_t divergence[t].
+ *   kdn_scale_rows: x *= *scale in place (a device scalar); returns without touching x when it is 1.
+ * Workspaces: the *_workspace_size entries, 256-byte aligned.
+ */
+int kdn_token_logprobs(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
+                       int64_t ignore_index, float* logps, float* row_stats, int64_t n, int64_t V, float temperature,
+                       void* stream);
+int kdn_token_logprobs_backward(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
+                                int64_t ignore_index, const float* row_stats, const float* dlogps, void* dlogits,
+                                int64_t ld_d, int64_t n, int64_t V, float temperature, void* stream);
+size_t kdn_policy_loss_workspace_size(int64_t n);
+int kdn_policy_loss(const void* logits, int dtype, int64_t ld, const void* actions, int index_dtype,
+                    int64_t ignore_index, const float* old_logps, const float* advantages, const float* ref_logps,
+                    const float* weights, float clip_low, float clip_high, float kl_coef, float entropy_coef,
+                    float temperature, float* loss, float* logps, float* entropy, void* dlogits, int64_t ld_d,
+                    int64_t n, int64_t V, void* workspace, size_t workspace_bytes, void* stream);
+size_t kdn_preference_loss_workspace_size(int64_t n, int64_t pairs);
+int kdn_preference_loss(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
+                        int64_t ignore_index, const int64_t* cu_seqlens, int64_t pairs, const float* ref_logps,
+                        float beta, float label_smoothing, int length_normalised, float temperature, float* loss,
+                        float* log_ratios, float* logps, void* dlogits, int64_t ld_d, int64_t n, int64_t V,
+                        void* workspace, size_t workspace_bytes, void* stream);
+size_t kdn_distillation_loss_workspace_size(int64_t n);
+int kdn_distillation_loss(const void* logits, int dtype, int64_t ld, const void* teacher_logits, int teacher_dtype,
+                          const void* teacher_ids, int index_dtype, int32_t top, const float* teacher_lse,
+                          const float* weights, float temperature, float* loss, float* divergence, void* dlogits,
+                          int64_t ld_d, int64_t n, int64_t V, void* workspace, size_t workspace_bytes, void* stream);
+int kdn_scale_rows(void* x, int dtype, int64_t ld, int64_t n, int64_t V, const float* scale, void* stream);
+
+/*
  * Layout change of a ragged serving batch (no reference counterpart; the reference packs
  * requests the same way, serving/vllm_ragged_batching.py:57-67, then loops over them).
  * Element (sequence i, token t, head h) of the packed [total_tokens, H, row] tensor sits at

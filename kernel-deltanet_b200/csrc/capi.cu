@@ -122,6 +122,56 @@ int check_affine_dims(int64_t batch, int32_t D, int32_t dv, bool need_dv) {
   return KDN_OK;
 }
 
+// arguments that every loss over logits shares
+int check_loss_rows(const void* logits, int dtype, int64_t ld, const void* dlogits, int64_t ld_d, int64_t n, int64_t V,
+                    int index_dtype, float temperature) {
+  if (!valid_dtype(dtype)) return fail(KDN_ERR_INVALID, "bad dtype");
+  if (index_dtype != KDN_INDEX_I32 && index_dtype != KDN_INDEX_I64) return fail(KDN_ERR_INVALID, "bad index dtype");
+  if (n < 0 || n > 0x7fffffff) return fail(KDN_ERR_INVALID, "n=%lld outside [0, 2^31)", (long long)n);
+  if (V < 1 || V > (int64_t(1) << 30)) return fail(KDN_ERR_INVALID, "V=%lld outside [1, 2^30]", (long long)V);
+  if (!(temperature > 0.f) || temperature > 3e38f)
+    return fail(KDN_ERR_INVALID, "temperature must be positive and finite");
+  if (n == 0) return KDN_OK;
+  if (!logits) return fail(KDN_ERR_INVALID, "logits is NULL");
+  if (ld < V) return fail(KDN_ERR_INVALID, "ld=%lld below V=%lld", (long long)ld, (long long)V);
+  const size_t size = dtype == KDN_DTYPE_BF16 ? 2 : 4;
+  if (!aligned(logits, size)) return fail(KDN_ERR_INVALID, "logits must be aligned to their element size");
+  if (dlogits) {
+    if (ld_d < V) return fail(KDN_ERR_INVALID, "ld_d=%lld below V=%lld", (long long)ld_d, (long long)V);
+    if (!aligned(dlogits, size)) return fail(KDN_ERR_INVALID, "dlogits must be aligned to its element size");
+    if (overlaps(logits, size * (size_t(n - 1) * ld + V), dlogits, size * (size_t(n - 1) * ld_d + V)))
+      return fail(KDN_ERR_INVALID, "dlogits overlaps logits");
+  }
+  return KDN_OK;
+}
+
+kdn::LossRows loss_rows(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
+                        int64_t ignore_index, void* dlogits, int64_t ld_d, int64_t n, int64_t V, float temperature) {
+  kdn::LossRows a{};
+  a.logits = logits;
+  a.dtype = dtype;
+  a.ld = ld;
+  a.labels = labels;
+  a.index_dtype = index_dtype;
+  a.ignore_index = ignore_index;
+  a.n = n;
+  a.V = V;
+  a.k = float(1.4426950408889634 / double(temperature));
+  a.inv_t = float(1.0 / double(temperature));
+  a.dlogits = dlogits;
+  a.ld_d = ld_d;
+  return a;
+}
+
+size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
+
+int check_loss_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (!workspace || bytes < need)
+    return fail(KDN_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed", bytes, need);
+  if (!aligned(workspace, 256)) return fail(KDN_ERR_INVALID, "workspace must be 256-byte aligned");
+  return KDN_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -820,6 +870,166 @@ int kdn_fork_state(void* states, int64_t num_slots, int64_t bytes_per_slot, int6
   return ok();
 }
 
+int kdn_token_logprobs(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
+                       int64_t ignore_index, float* logps, float* row_stats, int64_t n, int64_t V, float temperature,
+                       void* stream) {
+  if (int rc = check_loss_rows(logits, dtype, ld, nullptr, 0, n, V, index_dtype, temperature)) return rc;
+  if (n == 0) return ok();
+  if (!labels || !logps) return fail(KDN_ERR_INVALID, "labels/logps is NULL");
+  kdn::LossRows a = loss_rows(logits, dtype, ld, labels, index_dtype, ignore_index, nullptr, 0, n, V, temperature);
+  a.logps = logps;
+  a.stats = row_stats;
+  cudaError_t e = kdn::launch_token_logprobs(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "token log-probability launch");
+  return ok();
+}
+
+int kdn_token_logprobs_backward(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
+                                int64_t ignore_index, const float* row_stats, const float* dlogps, void* dlogits,
+                                int64_t ld_d, int64_t n, int64_t V, float temperature, void* stream) {
+  if (int rc = check_loss_rows(logits, dtype, ld, dlogits, ld_d, n, V, index_dtype, temperature)) return rc;
+  if (n == 0) return ok();
+  if (!labels || !row_stats || !dlogps || !dlogits)
+    return fail(KDN_ERR_INVALID, "labels/row_stats/dlogps/dlogits is NULL");
+  kdn::LossRows a = loss_rows(logits, dtype, ld, labels, index_dtype, ignore_index, dlogits, ld_d, n, V, temperature);
+  a.stats = const_cast<float*>(row_stats);
+  cudaError_t e = kdn::launch_token_logprobs_backward(a, dlogps, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "token log-probability backward launch");
+  return ok();
+}
+
+size_t kdn_policy_loss_workspace_size(int64_t n) { return n < 0 ? 0 : 256 + align256(sizeof(float) * size_t(n)); }
+
+int kdn_policy_loss(const void* logits, int dtype, int64_t ld, const void* actions, int index_dtype,
+                    int64_t ignore_index, const float* old_logps, const float* advantages, const float* ref_logps,
+                    const float* weights, float clip_low, float clip_high, float kl_coef, float entropy_coef,
+                    float temperature, float* loss, float* logps, float* entropy, void* dlogits, int64_t ld_d,
+                    int64_t n, int64_t V, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_loss_rows(logits, dtype, ld, dlogits, ld_d, n, V, index_dtype, temperature)) return rc;
+  if (!(clip_low >= 0.f && clip_low <= 1.f) || !(clip_high >= 0.f))
+    return fail(KDN_ERR_INVALID, "clip_low must be in [0, 1] and clip_high not negative");
+  if (!(kl_coef == kl_coef) || !(entropy_coef == entropy_coef)) return fail(KDN_ERR_INVALID, "a coefficient is NaN");
+  if (kl_coef != 0.f && !ref_logps && n > 0) return fail(KDN_ERR_INVALID, "kl_coef without ref_logps");
+  if (!loss) return fail(KDN_ERR_INVALID, "loss is NULL");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (n == 0) {
+    cudaError_t e = cudaMemsetAsync(loss, 0, sizeof(float), st);
+    if (e != cudaSuccess) return cuda_fail(e, "zero loss");
+    return ok();
+  }
+  if (!actions || !old_logps || !advantages || !logps)
+    return fail(KDN_ERR_INVALID, "actions/old_logps/advantages/logps is NULL");
+  if (int rc = check_loss_workspace(workspace, workspace_bytes, kdn_policy_loss_workspace_size(n))) return rc;
+  kdn::LossRows a = loss_rows(logits, dtype, ld, actions, index_dtype, ignore_index, dlogits, ld_d, n, V, temperature);
+  a.logps = logps;
+  kdn::PolicyTerms t{};
+  t.old_logps = old_logps;
+  t.advantages = advantages;
+  t.ref_logps = kl_coef != 0.f ? ref_logps : nullptr;
+  t.weights = weights;
+  t.scale = static_cast<float*>(workspace);
+  t.clip_low = clip_low;
+  t.clip_high = clip_high;
+  t.kl_coef = kl_coef;
+  t.entropy_coef = entropy_coef;
+  t.row_loss = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  t.entropy = entropy;
+  cudaError_t e = kdn::launch_policy_loss(a, t, loss, st);
+  if (e != cudaSuccess) return cuda_fail(e, "policy loss launch");
+  return ok();
+}
+
+size_t kdn_preference_loss_workspace_size(int64_t n, int64_t pairs) {
+  if (n < 0 || pairs < 1) return 0;
+  return align256(2 * sizeof(float) * size_t(n)) + align256(sizeof(float) * size_t(n)) +
+         align256(sizeof(float) * size_t(pairs));
+}
+
+int kdn_preference_loss(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
+                        int64_t ignore_index, const int64_t* cu_seqlens, int64_t pairs, const float* ref_logps,
+                        float beta, float label_smoothing, int length_normalised, float temperature, float* loss,
+                        float* log_ratios, float* logps, void* dlogits, int64_t ld_d, int64_t n, int64_t V,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_loss_rows(logits, dtype, ld, dlogits, ld_d, n, V, index_dtype, temperature)) return rc;
+  if (pairs < 1 || pairs > 0x3fffffff) return fail(KDN_ERR_INVALID, "pairs=%lld outside [1, 2^30)", (long long)pairs);
+  if (!(beta > 0.f) || beta > 3e38f) return fail(KDN_ERR_INVALID, "beta must be positive and finite");
+  if (!(label_smoothing >= 0.f && label_smoothing < 0.5f))
+    return fail(KDN_ERR_INVALID, "label_smoothing must be in [0, 0.5)");
+  if (!loss || !log_ratios || !cu_seqlens) return fail(KDN_ERR_INVALID, "loss/log_ratios/cu_seqlens is NULL");
+  if (n > 0 && (!labels || !logps)) return fail(KDN_ERR_INVALID, "labels/logps is NULL");
+  if (int rc = check_loss_workspace(workspace, workspace_bytes, kdn_preference_loss_workspace_size(n, pairs))) return rc;
+  kdn::LossRows a = loss_rows(logits, dtype, ld, labels, index_dtype, ignore_index, dlogits, ld_d, n, V, temperature);
+  char* ws = static_cast<char*>(workspace);
+  a.logps = logps;
+  a.stats = reinterpret_cast<float*>(ws);
+  ws += align256(2 * sizeof(float) * size_t(n));
+  kdn::PairTerms t{};
+  t.coef = reinterpret_cast<float*>(ws);
+  t.pair_loss = reinterpret_cast<float*>(ws + align256(sizeof(float) * size_t(n)));
+  t.cu = cu_seqlens;
+  t.pairs = pairs;
+  t.n = n;
+  t.labels = labels;
+  t.index_dtype = index_dtype;
+  t.ignore_index = ignore_index;
+  t.logps = logps;
+  t.ref = ref_logps;
+  t.beta = beta;
+  t.smoothing = label_smoothing;
+  t.normalise = length_normalised != 0;
+  t.log_ratios = log_ratios;
+  cudaError_t e = kdn::launch_preference_loss(a, t, loss, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "preference loss launch");
+  return ok();
+}
+
+size_t kdn_distillation_loss_workspace_size(int64_t n) { return kdn_policy_loss_workspace_size(n); }
+
+int kdn_distillation_loss(const void* logits, int dtype, int64_t ld, const void* teacher_logits, int teacher_dtype,
+                          const void* teacher_ids, int index_dtype, int32_t top, const float* teacher_lse,
+                          const float* weights, float temperature, float* loss, float* divergence, void* dlogits,
+                          int64_t ld_d, int64_t n, int64_t V, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_loss_rows(logits, dtype, ld, dlogits, ld_d, n, V, index_dtype, temperature)) return rc;
+  if (!valid_dtype(teacher_dtype)) return fail(KDN_ERR_INVALID, "bad dtype");
+  if (top < 1) return fail(KDN_ERR_INVALID, "top=%d < 1", top);
+  if (top > 1024) return fail(KDN_ERR_UNSUPPORTED, "top=%d: at most 1024 teacher entries a row", top);
+  if (!loss) return fail(KDN_ERR_INVALID, "loss is NULL");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (n == 0) {
+    cudaError_t e = cudaMemsetAsync(loss, 0, sizeof(float), st);
+    if (e != cudaSuccess) return cuda_fail(e, "zero loss");
+    return ok();
+  }
+  if (!teacher_logits || !teacher_ids || !divergence)
+    return fail(KDN_ERR_INVALID, "teacher_logits/teacher_ids/divergence is NULL");
+  if (int rc = check_loss_workspace(workspace, workspace_bytes, kdn_distillation_loss_workspace_size(n))) return rc;
+  kdn::LossRows a = loss_rows(logits, dtype, ld, nullptr, index_dtype, 0, dlogits, ld_d, n, V, temperature);
+  kdn::DistillTerms t{};
+  t.logits = teacher_logits;
+  t.dtype = teacher_dtype;
+  t.ids = teacher_ids;
+  t.K = top;
+  t.lse = teacher_lse;
+  t.weights = weights;
+  t.scale = static_cast<float*>(workspace);
+  t.temperature = temperature;
+  t.t2 = temperature * temperature;
+  t.row_loss = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  t.divergence = divergence;
+  cudaError_t e = kdn::launch_distillation_loss(a, t, loss, st);
+  if (e != cudaSuccess) return cuda_fail(e, "distillation loss launch");
+  return ok();
+}
+
+int kdn_scale_rows(void* x, int dtype, int64_t ld, int64_t n, int64_t V, const float* scale, void* stream) {
+  if (int rc = check_loss_rows(x, dtype, ld, nullptr, 0, n, V, KDN_INDEX_I64, 1.f)) return rc;
+  if (n == 0) return ok();
+  if (!scale) return fail(KDN_ERR_INVALID, "scale is NULL");
+  cudaError_t e = kdn::launch_scale_rows(x, dtype, ld, n, V, scale, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "scale launch");
+  return ok();
+}
+
 int kdn_device_error(void* stream, int* code_out) {
   if (!code_out) return fail(KDN_ERR_INVALID, "code_out is NULL");
   int code = 0, code_tc = 0, code_split = 0;
@@ -838,9 +1048,13 @@ int kdn_device_error(void* stream, int* code_out) {
   int code_attn = 0;
   e = kdn::attn_read_error(static_cast<cudaStream_t>(stream), &code_attn);
   if (e != cudaSuccess) return cuda_fail(e, "device error read");
-  *code_out = code ? code
-                   : (code_tc ? code_tc
-                              : (code_split ? code_split : (code_proj ? code_proj : (code_lift ? code_lift : code_attn))));
+  int code_loss = 0;
+  e = kdn::loss_read_error(static_cast<cudaStream_t>(stream), &code_loss);
+  if (e != cudaSuccess) return cuda_fail(e, "device error read");
+  const int codes[] = {code, code_tc, code_split, code_proj, code_lift, code_attn, code_loss};
+  *code_out = 0;
+  for (int c : codes)
+    if (*code_out == 0) *code_out = c;
   return ok();
 }
 

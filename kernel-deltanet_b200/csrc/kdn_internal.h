@@ -180,6 +180,69 @@ cudaError_t launch_decode_attn(const void* q, const void* k_cache, const void* v
                                void* out, int dt, int64_t B, int H, int64_t max_len, float* part,
                                cudaStream_t stream);
 
+// ---------------------------------------------------------------- losses.cu
+// The rows of logits that a loss reads, and where their gradient goes.
+struct LossRows {
+  const void* logits;  // [n, V], rows ld elements apart
+  int dtype;
+  int64_t ld;
+  const void* labels;  // [n] (null for the distillation loss)
+  int index_dtype;
+  int64_t ignore_index;
+  int64_t n, V;
+  float k;      // log2(e) / temperature
+  float inv_t;  // 1 / temperature
+  float* logps;        // [n]
+  float* stats;        // [n, 2]: largest logit, sum of e^((z - largest) / T); may be null
+  void* dlogits;       // [n, V], rows ld_d elements apart; null: no gradient
+  int64_t ld_d;
+  float* coef_zero;    // [n] set to zero by the forward pass; may be null
+};
+struct PolicyTerms {
+  const float* old_logps;   // [n]
+  const float* advantages;  // [n]
+  const float* ref_logps;   // [n] or null
+  const float* weights;     // [n] or null: *scale
+  const float* scale;
+  float clip_low, clip_high, kl_coef, entropy_coef;
+  float* row_loss;  // [n] weight x loss of each row (null: no loss, log-probabilities only)
+  float* entropy;   // [n] or null
+};
+struct PairTerms {
+  const int64_t* cu;  // [2 pairs + 1]
+  int64_t pairs, n;
+  const void* labels;
+  int index_dtype;
+  int64_t ignore_index;
+  const float* logps;  // [n]
+  const float* ref;    // [n] or null
+  float beta, smoothing;
+  bool normalise;
+  float* log_ratios;  // [2 pairs]
+  float* pair_loss;   // [pairs]
+  float* coef;        // [n] d loss / d logp
+};
+struct DistillTerms {
+  const void* logits;  // [n, K] teacher logits (dtype)
+  int dtype;
+  const void* ids;     // [n, K] (the rows' index_dtype)
+  int K;
+  const float* lse;      // [n] or null: the teacher renormalised over its K entries
+  const float* weights;  // [n] or null: *scale
+  const float* scale;
+  float temperature, t2;  // T, T^2
+  float* row_loss;        // [n]
+  float* divergence;      // [n]
+};
+cudaError_t launch_token_logprobs(const LossRows& a, cudaStream_t stream);
+cudaError_t launch_token_logprobs_backward(const LossRows& a, const float* dlogps, cudaStream_t stream);
+cudaError_t launch_policy_loss(const LossRows& a, const PolicyTerms& t, float* loss, cudaStream_t stream);
+cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, float* loss, cudaStream_t stream);
+cudaError_t launch_distillation_loss(const LossRows& a, const DistillTerms& t, float* loss, cudaStream_t stream);
+cudaError_t launch_scale_rows(void* x, int dtype, int64_t ld, int64_t n, int64_t V, const float* scale,
+                              cudaStream_t stream);
+cudaError_t loss_read_error(cudaStream_t stream, int* code);
+
 // ---------------------------------------------------------------- ragged.cu
 // rows of a packed [total, H, w] batch <-> per-sequence head-major [H, T_i, w] blocks
 cudaError_t launch_ragged_transpose(const void* src, void* dst, const void* cu_seqlens, int index_dtype,
