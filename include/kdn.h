@@ -374,7 +374,8 @@ int kdn_varlen_causal_attention(const void* q, const void* k_cache, const void* 
  *     negative ids are padding, and a row whose FIRST id is negative counts for nothing; an id >= V is skipped and
  *     recorded, code 1; an id given twice counts twice).  teacher_lse NULL: p = softmax of the row's entries / T; else
  *     p = e^(teacher / T - teacher_lse[t]) (log-sum-exp of the teacher's whole row / T) and what is left of the
- *     teacher's mass, 1 - sum p, is compared with the student's mass outside the ids as one more class.
+ *     teacher's mass, 1 - sum p, is compared with the student's mass outside the ids as one more class (where the
+ *     student has none the divergence is +inf and the gradient outside the ids zero).
  *     divergence[t] = KL(p || q), loss = T^2 sum_t w_t divergence[t].
  *   kdn_scale_rows: x *= *scale in place (a device scalar); returns without touching x when it is 1.
  * Workspaces: the *_workspace_size entries, 256-byte aligned.
@@ -505,7 +506,7 @@ int kdn_fork_state(void* states, int64_t num_slots, int64_t bytes_per_slot,
  * Synchronises `stream`.  *code_out = 0 when nothing was recorded; otherwise 1 = a slot,
  * length or offset out of range, 2 = fused tensor-core prefill wait, 3 = two-phase prefill
  * wait, 4 = decode wait, 5 = tensor-parallel projection wait, 6 = tensor-core lift wait,
- * 7 = anchor attention wait.
+ * 7 = anchor attention wait, 8 = losses over logits wait.
  */
 int kdn_device_error(void* stream, int* code_out);
 

@@ -127,7 +127,7 @@ int check_loss_rows(const void* logits, int dtype, int64_t ld, const void* dlogi
                     int index_dtype, float temperature) {
   if (!valid_dtype(dtype)) return fail(KDN_ERR_INVALID, "bad dtype");
   if (index_dtype != KDN_INDEX_I32 && index_dtype != KDN_INDEX_I64) return fail(KDN_ERR_INVALID, "bad index dtype");
-  if (n < 0 || n > 0x7fffffff) return fail(KDN_ERR_INVALID, "n=%lld outside [0, 2^31)", (long long)n);
+  if (n < 0 || n >= (int64_t(1) << 28)) return fail(KDN_ERR_INVALID, "n=%lld outside [0, 2^28)", (long long)n);
   if (V < 1 || V > (int64_t(1) << 30)) return fail(KDN_ERR_INVALID, "V=%lld outside [1, 2^30]", (long long)V);
   if (!(temperature > 0.f) || temperature > 3e38f)
     return fail(KDN_ERR_INVALID, "temperature must be positive and finite");
@@ -156,6 +156,7 @@ kdn::LossRows loss_rows(const void* logits, int dtype, int64_t ld, const void* l
   a.ignore_index = ignore_index;
   a.n = n;
   a.V = V;
+  a.temperature = temperature;
   a.k = float(1.4426950408889634 / double(temperature));
   a.inv_t = float(1.0 / double(temperature));
   a.dlogits = dlogits;
@@ -1012,7 +1013,6 @@ int kdn_distillation_loss(const void* logits, int dtype, int64_t ld, const void*
   t.lse = teacher_lse;
   t.weights = weights;
   t.scale = static_cast<float*>(workspace);
-  t.temperature = temperature;
   t.t2 = temperature * temperature;
   t.row_loss = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
   t.divergence = divergence;

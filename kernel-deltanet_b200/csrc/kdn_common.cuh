@@ -133,5 +133,6 @@ constexpr int kErrDecodeWaitTimeout = 4; // decode: a bounded wait gave up
 constexpr int kErrProjWaitTimeout = 5;   // tensor-parallel projection: a bounded wait gave up
 constexpr int kErrLiftWaitTimeout = 6;   // tensor-core lift: a bounded wait gave up
 constexpr int kErrAttnWaitTimeout = 7;   // anchor attention: a bounded wait gave up
+constexpr int kErrLossWaitTimeout = 8;   // losses over logits: a bounded wait gave up
 
 }  // namespace kdn

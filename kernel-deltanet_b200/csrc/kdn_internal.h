@@ -190,6 +190,7 @@ struct LossRows {
   int index_dtype;
   int64_t ignore_index;
   int64_t n, V;
+  float temperature;
   float k;      // log2(e) / temperature
   float inv_t;  // 1 / temperature
   float* logps;        // [n]
@@ -230,7 +231,7 @@ struct DistillTerms {
   const float* lse;      // [n] or null: the teacher renormalised over its K entries
   const float* weights;  // [n] or null: *scale
   const float* scale;
-  float temperature, t2;  // T, T^2
+  float t2;  // T^2
   float* row_loss;        // [n]
   float* divergence;      // [n]
 };

@@ -11,12 +11,20 @@
 // value.  Where every logit of a row is
 // -inf (or one is NaN or +inf) the row's results are NaN, as the formula gives.
 //
-// One CTA per row, two passes over it: the row's statistics, then (where a gradient is asked for) the
-// gradient.
+// Two kinds of kernels.  In the first a row belongs to a warp, a CTA or a cluster of up to 8 CTAs, each with a
+// contiguous share of the row's 16-byte vectors.  A share of up to 8 vectors a thread stays in registers between the two
+// passes over it (statistics, then gradient), so the logits are read from memory once and the gradient is written once;
+// the row's statistics are merged through warp shuffles, one barrier, and (in a cluster) one exchange through
+// distributed shared memory.  Longer shares are taken in rounds and read again for the gradient.  The second, for the
+// losses with a gradient over many long rows, streams them through a ring in shared memory: policy_stream_kernel.
 #include <math.h>
+
+#include <algorithm>
+#include <type_traits>
 
 #include "kdn_common.cuh"
 #include "kdn_internal.h"
+#include "tc_prims.cuh"
 
 namespace kdn {
 
@@ -25,12 +33,47 @@ __device__ int g_loss_error;
 namespace {
 
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kThreads = 256;
+constexpr int kMaxCluster = 8;
+constexpr int kNV = 8;  // vectors of a share that a thread keeps in registers
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tsub.rn.f32x2 z, x, y;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
 }
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -43,45 +86,256 @@ __device__ __forceinline__ int64_t ld_index(const void* p, int index_dtype, int6
                                       : int64_t(static_cast<const int32_t*>(p)[i]);
 }
 
-__device__ __forceinline__ float block_max(float v, float* red) {
+// ------------------------------------------------------------------------------------- 16-byte vectors of a row
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int E = 4;
+  static constexpr uint32_t kFill = 0xff800000u;  // -inf
+  static __device__ __forceinline__ float2 pair(const uint4& v, int i) {
+    return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
+                  : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+  }
+  static __device__ __forceinline__ float2 minus(const uint4& v, int i, float m) {
+    return sub2(pair(v, i), make_float2(m, m));
+  }
+  template <int N>
+  static __device__ __forceinline__ float largest(const uint4* v) {
+    float m = -INFINITY;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < int(blockDim.x >> 5); ++w) v = fmaxf(v, red[w]);
+    for (int i = 0; i < N; ++i)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v[i].x), __uint_as_float(v[i].y)),
+                         fmaxf(__uint_as_float(v[i].z), __uint_as_float(v[i].w))));
+    return m;
+  }
+  static __device__ __forceinline__ uint4 pack(const float2* f) {
+    return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x),
+                      __float_as_uint(f[1].y));
+  }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int E = 8;
+  static constexpr uint32_t kFill = 0xff80ff80u;
+  static __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+  }
+  static __device__ __forceinline__ float2 pair(const uint4& v, int i) {
+    const uint32_t w = word(v, i);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  // elements 2i, 2i + 1 as fp32 less m: a subtraction takes a bf16 operand as it is
+  static __device__ __forceinline__ float2 minus(const uint4& v, int i, float m) {
+    float2 r;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.bf16 %0, l, %3;\n\tsub.rn.f32.bf16 %1, h, %3;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(word(v, i)), "f"(m));
+    return r;
+  }
+  template <int N>
+  static __device__ __forceinline__ float largest(const uint4* v) {
+    auto h = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    __nv_bfloat162 m = __hmax2(__hmax2(h(v[0].x), h(v[0].y)), __hmax2(h(v[0].z), h(v[0].w)));
+#pragma unroll
+    for (int i = 1; i < N; ++i)
+      m = __hmax2(m, __hmax2(__hmax2(h(v[i].x), h(v[i].y)), __hmax2(h(v[i].z), h(v[i].w))));
+    return fmaxf(fmaxf(__low2float(m), __high2float(m)), -INFINITY);  // NaN only where every one is: -inf
+  }
+  static __device__ __forceinline__ uint4 pack(const float2* f) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 t = __float22bfloat162_rn(f[i]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
   return v;
 }
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.f;
-  for (int w = 0; w < int(blockDim.x >> 5); ++w) v += red[w];
-  return v;
+// the vector that starts at element j0 of a row of V (one that reaches over an end of the row); elements outside
+// the row are -inf
+template <typename T>
+__device__ __noinline__ uint4 load_edge(const T* z, int j0, int V) {
+  uint32_t w[4] = {Vec<T>::kFill, Vec<T>::kFill, Vec<T>::kFill, Vec<T>::kFill};
+#pragma unroll
+  for (int e = 0; e < Vec<T>::E; ++e) {
+    const int j = j0 + e;
+    if (j < 0 || j >= V) continue;
+    if constexpr (sizeof(T) == 4) {
+      w[e] = __float_as_uint(z[j]);
+    } else {
+      const uint32_t b = reinterpret_cast<const uint16_t*>(z)[j];
+      w[e / 2] = (e & 1) ? ((w[e / 2] & 0xffffu) | (b << 16)) : ((w[e / 2] & 0xffff0000u) | b);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ double block_sum_f64(double v, double* red) {
+// such a vector read whole: what lies outside the row becomes -inf / is not stored
+template <typename T>
+__device__ __noinline__ uint4 mask_edge(uint4 v, int j0, int V) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int e = 0; e < Vec<T>::E; ++e) {
+    if (j0 + e >= 0 && j0 + e < V) continue;
+    if constexpr (sizeof(T) == 4)
+      w[e] = Vec<T>::kFill;
+    else
+      w[e / 2] = (e & 1) ? ((w[e / 2] & 0xffffu) | 0xff800000u) : ((w[e / 2] & 0xffff0000u) | 0xff80u);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __noinline__ void store_edge(T* dz, uint4 v, int j0, int V) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < Vec<T>::E; ++e) {
+    const int j = j0 + e;
+    if (j < 0 || j >= V) continue;
+    if constexpr (sizeof(T) == 4)
+      dz[j] = __uint_as_float(w[e]);
+    else
+      reinterpret_cast<uint16_t*>(dz)[j] = uint16_t((e & 1) ? w[e / 2] >> 16 : w[e / 2]);
+  }
+}
+
+// A CTA's share of a row: vector vi holds the row's elements [vi E - off, vi E - off + E), off the row's start
+// within its first 16 bytes; vectors [v0, v1) are the share.
+template <typename T>
+struct Share {
+  static constexpr int E = Vec<T>::E;
+  const T* z;
+  T* dz;
+  int off, V, v0, v1;
+  bool same;  // the gradient's row starts at the same place within 16 bytes
+
+  __device__ __forceinline__ Share(const LossRows& a, int64_t r, int rank, int parts) {
+    z = static_cast<const T*>(a.logits) + r * a.ld;
+    dz = a.dlogits ? static_cast<T*>(a.dlogits) + r * a.ld_d : nullptr;
+    V = int(a.V);
+    const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>(z)) & 15u;
+    off = int(at / sizeof(T));
+    same = (uint32_t(reinterpret_cast<uintptr_t>(dz)) & 15u) == at;
+    const int nvec = (off + V + E - 1) / E, per = (nvec + parts - 1) / parts;
+    v0 = min(rank * per, nvec);
+    v1 = min(v0 + per, nvec);
+  }
+  __device__ __forceinline__ bool whole(int vi) const { return vi * E >= off && (vi + 1) * E - off <= V; }
+  __device__ __forceinline__ uint4 load(int vi) const {
+    if (whole(vi)) return ld_stream(z + (vi * E - off));
+    return load_edge(z, vi * E - off, V);
+  }
+  __device__ __forceinline__ void store(int vi, const float2* g) const {
+    if (same && whole(vi)) {
+      *reinterpret_cast<uint4*>(dz + (vi * E - off)) = Vec<T>::pack(g);
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int j = vi * E - off + e;
+      if (j >= 0 && j < V) from_f32(dz + j, (e & 1) ? g[e / 2].y : g[e / 2].x);
+    }
+  }
+  template <int NT>
+  __device__ __forceinline__ void zero(int tid) const {
+    const float2 g[4] = {};
+    for (int vi = v0 + tid; vi < v1; vi += NT) store(vi, g);
+  }
+};
+
+// The CTAs of the kernels that keep a row in registers: NT threads a row (32: four rows to a CTA).
+template <int NT>
+struct Cta {
+  static constexpr int kThreads = NT < 128 ? 128 : NT, kRows = kThreads / NT;
+  static __device__ __forceinline__ int64_t row(int parts) {
+    return int64_t(blockIdx.x / unsigned(parts)) * kRows + threadIdx.x / NT;
+  }
+};
+
+// Largest logit m, sum of exponentials below it, and a second sum (see its use) of a part of a row.
+struct Stats {
+  float m, s, u;
+};
+
+// The statistics of two parts together.  kMoment: u is sum e^d d (base 2), which a change of m shifts; else a sum
+// like s.  A part without a finite logit has m = -inf and sums of zero (or NaN) and is left as it is.
+template <bool kMoment>
+__device__ __forceinline__ void rescale(Stats& a, float m, float k) {
+  if (a.m == m) return;
+  const float d = (a.m - m) * k, f = ex2(d);
+  if constexpr (kMoment)
+    a.u = f == 0.f ? 0.f : f * fmaf(a.s, d, a.u);
+  else
+    a.u *= f;
+  a.s *= f;
+  a.m = m;
+}
+
+// the statistics of a warp's lanes together
+template <bool kMoment>
+__device__ __forceinline__ Stats merge_warp(Stats a, float k) {
+  float m = a.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  rescale<kMoment>(a, m, k);
+  a.s = warp_sum(a.s);
+  a.u = warp_sum(a.u);
+  return a;
+}
+
+// ... of `count` <= 64 parts in shared memory, by every warp that asks
+template <bool kMoment>
+__device__ __forceinline__ Stats merge_parts(const float4* p, int count, float k) {
+  const int lane = threadIdx.x & 31;
+  const float4 t = lane < count ? p[lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  Stats a{t.x, t.y, t.z};
+  if (count > 32 && lane + 32 < count) {
+    Stats b{p[lane + 32].x, p[lane + 32].y, p[lane + 32].z};
+    const float m = fmaxf(a.m, b.m);
+    rescale<kMoment>(a, m, k);
+    rescale<kMoment>(b, m, k);
+    a.s += b.s;
+    a.u += b.u;
+  }
+  return merge_warp<kMoment>(a, k);
+}
+
+// ... of all threads of the row's cluster
+template <int NT, bool kMoment>
+__device__ __forceinline__ Stats merge_rows(Stats a, float k, int rank, int parts) {
+  a = merge_warp<kMoment>(a, k);
+  if constexpr (NT == 32) return a;
+  __shared__ float4 part[NT / 32];
+  __shared__ float4 remote[kMaxCluster];
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float4(a.m, a.s, a.u, 0.f);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.0;
-  for (int w = 0; w < int(blockDim.x >> 5); ++w) v += red[w];
-  return v;
+  a = merge_parts<kMoment>(part, NT / 32, k);
+  if (parts > 1) {
+    if (threadIdx.x < unsigned(parts))
+      tc::st_cluster_v4(tc::mapa(tc::smem_u32(&remote[rank]), threadIdx.x), a.m, a.s, a.u, 0.f);
+    tc::cluster_arrive();
+    tc::cluster_wait();
+    a = merge_parts<kMoment>(remote, parts, k);
+  }
+  return a;
 }
 
 // the label of a row, or -1 for a row that counts for nothing (its label is ignore_index; a label outside
 // the vocabulary is recorded and treated the same way)
-__device__ __forceinline__ int64_t row_label(const LossRows& a, int64_t r) {
+__device__ __forceinline__ int64_t row_label(const LossRows& a, int64_t r, bool record) {
   const int64_t y = ld_index(a.labels, a.index_dtype, r);
   if (y == a.ignore_index) return -1;
   if (y < 0 || y >= a.V) {
-    if (threadIdx.x == 0) record_device_error(&g_loss_error, kErrSlotOutOfRange);
+    if (record) record_device_error(&g_loss_error, kErrSlotOutOfRange);
     return -1;
   }
   return y;
@@ -95,15 +349,23 @@ struct PolicyRow {
 //   l = -min(r A, clip(r, 1 - lo, 1 + hi) A) + c_kl (e^g - 1 - g) - c_H H,   g = ref - logp,
 // where e^g - 1 - g >= 0 estimates KL(policy || reference) from the policy's own sample.  The gradient of the
 // first term is -r A where the unclipped product is the smaller (or the two are equal), else zero.
-__device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, int64_t r, float logp, float H) {
+struct PolicyIn {
+  float w, adv, old, ref;
+};
+__device__ __forceinline__ PolicyIn policy_inputs(const PolicyTerms& t, int64_t r) {
+  if (!t.row_loss) return PolicyIn{};
+  return PolicyIn{t.weights ? t.weights[r] : *t.scale, t.advantages[r], t.old_logps[r],
+                  t.ref_logps ? t.ref_logps[r] : 0.f};
+}
+__device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, const PolicyIn& in, float logp, float H) {
   PolicyRow p;
-  p.w = t.weights ? t.weights[r] : *t.scale;
-  const float adv = t.advantages[r], ratio = expf(logp - t.old_logps[r]);
+  p.w = in.w;
+  const float adv = in.adv, ratio = expf(logp - in.old);
   const float free = ratio * adv, clipped = fminf(fmaxf(ratio, 1.f - t.clip_low), 1.f + t.clip_high) * adv;
   float l = free <= clipped ? -free : -clipped;
   float d = free <= clipped ? -free : 0.f;
   if (t.ref_logps) {
-    const float g = t.ref_logps[r] - logp, em = expm1f(g);
+    const float g = in.ref - logp, em = expm1f(g);
     l = fmaf(t.kl_coef, em - g, l);
     d = fmaf(-t.kl_coef, em, d);
   }
@@ -113,186 +375,813 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, int64_t r,
   return p;
 }
 
-template <typename T>
-__device__ __forceinline__ void zero_row(T* out, int V) {
-  for (int j = threadIdx.x; j < V; j += kThreads) from_f32(out + j, 0.f);
-}
+// What the gradient of a row needs: dz_j = 2^d (A + B d) with d = (z_j - m) k, and dz_y.
+struct RowCoef {
+  float m, A, B, at_label;
+  int y;  // -1: the gradient is zero
+};
 
-// -------------------------------------------------------------------- token log-probabilities, policy loss
-template <typename T>
-__global__ void __launch_bounds__(kThreads) logp_kernel(LossRows a, PolicyTerms t) {
-  __shared__ float red[kThreads / 32];
-  const int64_t r = blockIdx.x;
-  const T* z = static_cast<const T*>(a.logits) + r * a.ld;
-  T* dz = a.dlogits ? static_cast<T*>(a.dlogits) + r * a.ld_d : nullptr;
-  const int V = int(a.V);
-  const int64_t y = row_label(a, r);
-  if (y < 0) {
-    if (threadIdx.x == 0) {
-      a.logps[r] = 0.f;
-      if (a.stats) a.stats[2 * r] = 0.f, a.stats[2 * r + 1] = 1.f;
-      if (a.coef_zero) a.coef_zero[r] = 0.f;
-      if (t.entropy) t.entropy[r] = 0.f;
-      if (t.row_loss) t.row_loss[r] = 0.f;
-    }
-    if (dz) zero_row(dz, V);
-    return;
-  }
-  float mx = -INFINITY;
-  for (int j = threadIdx.x; j < V; j += kThreads) mx = fmaxf(mx, to_f32(z[j]));
-  mx = block_max(mx, red);
-  float s = 0.f, u = 0.f;
-  for (int j = threadIdx.x; j < V; j += kThreads) {
-    const float d = (to_f32(z[j]) - mx) * a.k;
-    const float e = ex2(d);
-    s += e;
-    u = fmaf(e, fmaxf(d, -1000.f), u);
-  }
-  s = block_sum(s, red);
-  u = block_sum(u, red);
-  const float l2s = log2f(s);
-  const float logp = kLn2 * ((to_f32(z[y]) - mx) * a.k - l2s);
-  if (threadIdx.x == 0) {
+// From a row's statistics: its outputs (written where `write` is set) and the coefficients of its gradient.
+//   log q_j = ln 2 d_j - log s,   entropy H = -sum q log q = log s - ln 2 (sum e d) / s,
+//   dz_j = (w / T) (dl/dlogp (1[j = y] - q_j) + c_H q_j (log q_j + H)).
+template <bool kEntropy, int kGrad>
+__device__ __forceinline__ RowCoef finish_row(const LossRows& a, const PolicyTerms& t, const PolicyIn& in, int64_t r,
+                                              int y, float zy, const Stats& st, bool write) {
+  // to base e and with a division, not through k = log2(e) / T, whose rounding would show in a log-probability (and
+  // products rounded on their own, so that calls with and without a gradient give the same bits)
+  const float dy = __fmul_rn(zy - st.m, a.k), ls = logf(st.s);
+  const float logp = __fsub_rn(__fdiv_rn(zy - st.m, a.temperature), ls);
+  if (write) {
     a.logps[r] = logp;
-    if (a.stats) a.stats[2 * r] = mx, a.stats[2 * r + 1] = s;
+    if (a.stats) a.stats[2 * r] = st.m, a.stats[2 * r + 1] = st.s;
     if (a.coef_zero) a.coef_zero[r] = 0.f;
   }
-  if (!t.row_loss) return;
-  const float H = kLn2 * (l2s - u / s);
-  const PolicyRow p = policy_row(t, r, logp, H);
-  if (threadIdx.x == 0) {
+  RowCoef o{st.m, 0.f, 0.f, 0.f, -1};
+  if (!t.row_loss) return o;
+  const float H = kEntropy ? fmaf(-kLn2, st.u / st.s, ls) : 0.f;
+  const PolicyRow p = policy_row(t, in, logp, H);
+  if (write) {
     t.row_loss[r] = p.loss;
     if (t.entropy) t.entropy[r] = H;
   }
-  if (!dz) return;
-  if (p.w == 0.f) {
-    zero_row(dz, V);
-    return;
-  }
-  const float c = p.dlogp * a.inv_t, h = p.w * t.entropy_coef * a.inv_t;
-  const float A = (h * (H - kLn2 * l2s) - c) / s, B = h * kLn2 / s;
-  for (int j = threadIdx.x; j < V; j += kThreads) {
-    const float d = (to_f32(z[j]) - mx) * a.k;
-    float g = ex2(d) * fmaf(B, fmaxf(d, -1000.f), A);
-    if (j == y) g += c;
-    from_f32(dz + j, g);
+  if (kGrad == 0 || p.w == 0.f) return o;
+  const float c = p.dlogp * a.inv_t, h = kGrad == 2 ? p.w * t.entropy_coef * a.inv_t : 0.f;
+  o.y = y;
+  o.A = kGrad == 2 ? (h * (H - ls) - c) / st.s : -c / st.s;
+  o.B = h * kLn2 / st.s;
+  o.at_label = fmaf(ex2(dy), kGrad == 2 ? fmaf(o.B, fmaxf(dy, -1000.f), o.A) : o.A, c);
+  return o;
+}
+
+// the outputs of a row that counts for nothing
+__device__ __forceinline__ void finish_dead_row(const LossRows& a, const PolicyTerms& t, int64_t r) {
+  a.logps[r] = 0.f;
+  if (a.stats) a.stats[2 * r] = 0.f, a.stats[2 * r + 1] = 1.f;
+  if (a.coef_zero) a.coef_zero[r] = 0.f;
+  if (t.entropy) t.entropy[r] = 0.f;
+  if (t.row_loss) t.row_loss[r] = 0.f;
+}
+
+// the gradient of one vector of logits (but for the label's own term)
+template <typename T, int kGrad>
+__device__ __forceinline__ void vector_grad(const uint4& v, float m, float k, float A, float B, float2* g) {
+#pragma unroll
+  for (int j = 0; j < Vec<T>::E / 2; ++j) {
+    const float2 d = mul2(Vec<T>::minus(v, j, m), make_float2(k, k));
+    const float2 e = make_float2(ex2(d.x), ex2(d.y));
+    if constexpr (kGrad == 2)
+      g[j] = mul2(e, fma2(make_float2(B, B), make_float2(fmaxf(d.x, -1000.f), fmaxf(d.y, -1000.f)),
+                          make_float2(A, A)));
+    else
+      g[j] = mul2(e, make_float2(A, A));
   }
 }
 
-// d/dz of sum_t dlogps_t logp_t from the saved statistics
+// g[e] += c for an e that is not known at compile time
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logp_backward_kernel(LossRows a, const float* __restrict__ dlogps) {
-  const int64_t r = blockIdx.x;
-  const T* z = static_cast<const T*>(a.logits) + r * a.ld;
-  T* dz = static_cast<T*>(a.dlogits) + r * a.ld_d;
-  const int V = int(a.V);
-  const int64_t y = row_label(a, r);
-  const float c = y < 0 ? 0.f : dlogps[r] * a.inv_t;
-  if (c == 0.f) {
-    zero_row(dz, V);
+__device__ __forceinline__ void add_at(float2* g, int e, float c) {
+#pragma unroll
+  for (int j = 0; j < Vec<T>::E / 2; ++j) {
+    if (e == 2 * j) g[j].x += c;
+    if (e == 2 * j + 1) g[j].y += c;
+  }
+}
+
+// The statistics of N vectors: s = sum 2^d and (kMoment) u = sum 2^d d with d = (z - base) k.
+template <typename T, int N, bool kMoment>
+__device__ __forceinline__ void accumulate(const uint4* v, float base, float k, float& s_out, float& u_out) {
+  float2 s = make_float2(0.f, 0.f), u = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < Vec<T>::E / 2; ++j) {
+      const float2 d = mul2(Vec<T>::minus(v[i], j, base), make_float2(k, k));
+      const float2 e = make_float2(ex2(d.x), ex2(d.y));
+      s = add2(s, e);
+      if constexpr (kMoment)  // a logit of -inf adds 0 x -1000, not 0 x -inf
+        u = fma2(e, make_float2(fmaxf(d.x, -1000.f), fmaxf(d.y, -1000.f)), u);
+    }
+  s_out = s.x + s.y;
+  u_out = u.x + u.y;
+}
+
+// `st` with N more vectors
+template <typename T, int N, bool kMoment>
+__device__ __forceinline__ void add_vectors(Stats& st, const uint4* v, float k) {
+  const float m = fmaxf(st.m, Vec<T>::template largest<N>(v));
+  rescale<kMoment>(st, m, k);
+  float s, u;
+  accumulate<T, N, kMoment>(v, m == -INFINITY ? 0.f : m, k, s, u);  // without a finite logit: 2^-inf each
+  st.s += s;
+  st.u += u;
+}
+
+// -------------------------------------------------------------------- token log-probabilities, policy loss
+// kEntropy: the row's entropy is formed; kGrad: the gradient is (kGrad == 2: with the entropy's term).
+template <typename T, int NT, bool kEntropy, int kGrad>
+__global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
+    logp_kernel(LossRows a, PolicyTerms t, int parts) {
+  const int64_t r = Cta<NT>::row(parts);
+  if (r >= a.n) return;
+  const int rank = int(blockIdx.x % unsigned(parts));
+  const Share<T> w(a, r, rank, parts);
+  const int tid = int(threadIdx.x) % NT;
+  const bool first = rank == 0 && tid == 0;
+  const int64_t y = row_label(a, r, first);
+  if (y < 0) {  // the same for every CTA of the cluster
+    if (first) finish_dead_row(a, t, r);
+    if (kGrad) w.template zero<NT>(tid);
     return;
   }
-  const float mx = a.stats[2 * r], A = -c / a.stats[2 * r + 1];
-  for (int j = threadIdx.x; j < V; j += kThreads) {
-    float g = ex2((to_f32(z[j]) - mx) * a.k) * A;
-    if (j == y) g += c;
-    from_f32(dz + j, g);
+  if (parts > 1) tc::cluster_arrive();
+  const float zy = to_f32(w.z[y]);
+  const PolicyIn in = policy_inputs(t, r);
+  uint4 v[kNV];
+  auto load = [&](int at) {
+#pragma unroll
+    for (int i = 0; i < kNV; ++i) {
+      const int vi = at + tid + i * NT;
+      v[i] = vi < w.v1 ? w.load(vi) : make_uint4(Vec<T>::kFill, Vec<T>::kFill, Vec<T>::kFill, Vec<T>::kFill);
+    }
+  };
+  const int rounds = max(1, (w.v1 - w.v0 + NT * kNV - 1) / (NT * kNV));
+  Stats st{-INFINITY, 0.f, 0.f};
+  for (int q = 0; q < rounds; ++q) {
+    load(w.v0 + q * NT * kNV);
+    add_vectors<T, kNV, kEntropy>(st, v, a.k);
+  }
+  if (parts > 1) tc::cluster_wait();  // every CTA of the cluster runs: their shared memory may be written
+  st = merge_rows<NT, kEntropy>(st, a.k, rank, parts);
+  const RowCoef o = finish_row<kEntropy, kGrad>(a, t, in, r, int(y), zy, st, first);
+  if constexpr (kGrad != 0) {
+    if (o.y < 0) {
+      w.template zero<NT>(tid);
+      return;
+    }
+    const int vy = (int(y) + w.off) / Vec<T>::E;
+    for (int q = rounds - 1; q >= 0; --q) {
+      if (q < rounds - 1) load(w.v0 + q * NT * kNV);
+#pragma unroll
+      for (int i = 0; i < kNV; ++i) {
+        const int vi = w.v0 + q * NT * kNV + tid + i * NT;
+        if (vi >= w.v1) break;
+        float2 g[Vec<T>::E / 2];
+        vector_grad<T, kGrad>(v[i], o.m, a.k, o.A, o.B, g);
+        w.store(vi, g);
+        if (vi == vy) from_f32(w.dz + y, o.at_label);  // after this thread's own store of the vector
+      }
+    }
+  }
+}
+
+// d/dz of sum_t dlogps_t logp_t from the saved statistics: one read, one write, nothing to reduce
+template <typename T, int NT>
+__global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
+    logp_backward_kernel(LossRows a, const float* __restrict__ dlogps, int parts) {
+  const int64_t r = Cta<NT>::row(parts);
+  if (r >= a.n) return;
+  const int tid = int(threadIdx.x) % NT;
+  const Share<T> w(a, r, int(blockIdx.x % unsigned(parts)), parts);
+  const int64_t y = row_label(a, r, tid == 0);
+  const float c = y < 0 ? 0.f : dlogps[r] * a.inv_t;
+  if (c == 0.f) {
+    w.template zero<NT>(tid);
+    return;
+  }
+  const float m = a.stats[2 * r], A = -c / a.stats[2 * r + 1];
+  const int vy = (int(y) + w.off) / Vec<T>::E, ey = (int(y) + w.off) % Vec<T>::E;
+  for (int at = w.v0 + tid; at < w.v1; at += NT * kNV) {
+    uint4 v[kNV];
+#pragma unroll
+    for (int i = 0; i < kNV; ++i)
+      if (at + i * NT < w.v1) v[i] = w.load(at + i * NT);
+#pragma unroll
+    for (int i = 0; i < kNV; ++i) {
+      const int vi = at + i * NT;
+      if (vi >= w.v1) break;
+      float2 g[Vec<T>::E / 2];
+      vector_grad<T, 1>(v[i], m, a.k, A, 0.f, g);
+      if (vi == vy) add_at<T>(g, ey, c);
+      w.store(vi, g);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------- many rows: the streaming kernel
+// One resident CTA (or cluster) an SM takes rows as they come, and its warps have roles, so that reading, arithmetic
+// and writing of different rows overlap (with a CTA per row, the CTAs of an SM load together and compute together: a
+// 32000-entry bf16 row takes about 2100 cycles of ex2 for its statistics, 2100 for its gradient, and 5600 of memory
+// time at the measured copy rate):
+//   producer   takes the next group of rows (the grid has a cluster for each; a resident one cancels the launch of
+//              one that has not started and does its work instead, so SMs that met many ignored rows take more),
+//              reads their labels, queues them for the other roles, and copies the share of those that count into a
+//              ring of chunks in shared memory;
+//   statistics (8 warps) maximum and sums of every chunk as it arrives, then one partial result a warp;
+//              (in a cluster, to the shared memory of every CTA of it);
+//   control    (2 warps, row about) merges a row's partials, computes the loss, writes the row's outputs and
+//              publishes the coefficients of its gradient;
+//   gradient   (8 warps) reads the row's chunks once more from shared memory, writes the gradient, frees them.
+// Every wait is bounded; after one that gave up a role ends, kErrLossWaitTimeout is recorded, and the CTA returns
+// when its copies have landed.
+constexpr int kPer = 4;                // vectors that a thread of a role takes at a time
+constexpr int kBuf = 16;               // rows between a partial result and its use (8 in a cluster), see Exchange
+constexpr int kQueue = 32;             // rows between the producer and the last of the other roles
+constexpr int kRoleThreads = 256;      // of the statistics and of the gradient role
+constexpr int kRoleWarps = kRoleThreads / 32;
+constexpr int kControlWarps = 2;
+constexpr int kStreamThreads = 2 * kRoleThreads + 32 * (kControlWarps + 1);
+constexpr uint32_t kLossWaitLimit = 1u << 20;
+constexpr int kChunk = kPer * kRoleThreads;  // vectors: 16 KiB
+constexpr int kSlots = 13;                   // chunks of the ring
+constexpr size_t kRingBytes = size_t(kSlots) * kChunk * 16;
+
+struct __align__(16) QueuedRow {
+  int64_t row;  // -1: no more rows
+  int label;    // -1: the row counts for nothing (-2: its label lies outside the vocabulary)
+  int pad;
+};
+
+// What the roles pass on.  Rows that count use the buffers for partial results and coefficients in turn, 16 of them,
+// or 8 in a cluster.  They are free when they are written: with a gradient, the ring holds 13 rows at most (3 in a
+// cluster, where a share is more than 4 chunks), a row leaves it when its coefficients have been used, and another
+// CTA's control is at most that far behind its statistics; without, statistics wait for the control warps to be at
+// most half of the buffers behind.
+struct Exchange {
+  uint4 response;                                      // of a request for more rows
+  float4 part[kBuf / 2 * kRoleWarps * kMaxCluster];    // (m, s, u) of each statistics warp of the cluster
+  QueuedRow queue[kQueue];
+  RowCoef coef[kBuf];
+  int ticket[2];                         // the cluster's next group of rows, -1: none
+  uint64_t full[kSlots], empty[kSlots];
+  uint64_t part_full[kBuf], coef_full[kBuf];
+  uint64_t queue_full[kQueue], queue_empty[kQueue];
+  uint64_t response_full, ticket_full[2], ticket_free[2];
+};
+
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t a, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// arrive on the barrier at the same address of CTA `rank` of the cluster / wait for arrivals of other CTAs
+__device__ __forceinline__ void arrive_cluster(uint64_t* bar, uint32_t rank) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(tc::mapa(tc::smem_u32(bar), rank))
+               : "memory");
+}
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity) {
+  bool done = false;
+  for (uint32_t i = 0; i < kLossWaitLimit && !done; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(tc::smem_u32(bar)), "r"(parity)
+        : "memory");
+    done = ok != 0;
+  }
+  return __all_sync(0xffffffffu, done);
+}
+// a warp's bounded wait, the same answer in every lane
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, tc::mbar_wait_bounded(bar, parity, kLossWaitLimit));
+}
+
+// 16 bytes to the same place of CTA `rank` of the cluster, counted by the barrier of that CTA
+__device__ __forceinline__ void st_async(float4* p, uint64_t* bar, uint32_t rank, float a, float b, float c) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+                   tc::mapa(tc::smem_u32(p), rank)),
+               "f"(a), "f"(b), "f"(c), "f"(0.f), "r"(tc::mapa(tc::smem_u32(bar), rank))
+               : "memory");
+}
+
+// Asks for the launch of a cluster that has not started to be cancelled; the answer (16 bytes) completes `bar`.
+__device__ __forceinline__ void request_rows(uint4* response, uint64_t* bar) {
+  tc::mbar_arrive_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   tc::smem_u32(response)),
+               "r"(tc::smem_u32(bar))
+               : "memory");
+}
+// the first CTA of the cluster that was cancelled, or -1 when there was none left
+__device__ __forceinline__ int64_t requested_cta(const uint4* response) {
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\tld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(tc::smem_u32(response))
+      : "memory");
+  return got ? int64_t(x) : -1;
+}
+
+// A place in a circular buffer: its index and the parity of its current use.
+struct Place {
+  int size, i = 0;
+  uint32_t parity = 0;
+  bool wrapped = false;
+  __device__ __forceinline__ explicit Place(int n) : size(n) {}
+  __device__ __forceinline__ void next() {
+    if (++i == size) i = 0, parity ^= 1u, wrapped = true;
+  }
+};
+
+// a share of `per` vectors for every row, whatever its start within 16 bytes
+template <typename T>
+struct RowShare {
+  static constexpr int E = Vec<T>::E;
+  int off, v0, count;  // as Share; vectors of the share
+  bool ragged;         // an end of the row lies inside one of them
+  __device__ __forceinline__ RowShare(const T* z, int V, int per, int rank) {
+    off = int((uint32_t(reinterpret_cast<uintptr_t>(z)) & 15u) / sizeof(T));
+    const int nvec = (off + V + E - 1) / E;
+    v0 = rank * per;
+    count = max(0, min(per, nvec - v0));
+    ragged = (v0 == 0 && off > 0) || (v0 + count == nvec && (off + V) % E != 0);
+  }
+};
+
+// The next row of a role's walk through the queue.
+struct QueueReader {
+  Place at{kQueue};
+  __device__ __forceinline__ bool next(Exchange& x, QueuedRow& row) {
+    const bool ok = warp_wait(&x.queue_full[at.i], at.parity);
+    if (ok) row = x.queue[at.i];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&x.queue_empty[at.i]);
+    at.next();
+    return ok;
+  }
+};
+
+template <typename T, int kGrad>
+__global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRows a, PolicyTerms t, int group_rows,
+                                                                        int per, int parts) {
+  extern __shared__ __align__(128) uint8_t ring_mem[];
+  __shared__ Exchange x;
+  constexpr int E = Vec<T>::E;
+  const int tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+  const int rank = int(blockIdx.x % unsigned(parts)), V = int(a.V);
+  const uint32_t ring = tc::smem_u32(ring_mem);
+  const T* logits = static_cast<const T*>(a.logits);
+  const uint32_t part_bytes = uint32_t(kRoleWarps * parts) * 16u;
+  if (tid < 64) {  // a few barriers a thread
+    if (tid < kSlots) {
+      tc::mbar_init(&x.full[tid], 1);
+      tc::mbar_init(&x.empty[tid], kRoleWarps);
+    }
+    if (tid < kBuf) {
+      tc::mbar_init(&x.part_full[tid], parts == 1 ? kRoleWarps : 1);
+      if (parts > 1) tc::mbar_arrive_expect_tx(&x.part_full[tid], part_bytes);
+      tc::mbar_init(&x.coef_full[tid], 1);
+    }
+    if (tid >= 32) {
+      tc::mbar_init(&x.queue_full[tid - 32], 1);
+      tc::mbar_init(&x.queue_empty[tid - 32], (kGrad ? 2 : 1) * kRoleWarps + kControlWarps);
+    }
+    if (tid == 16) tc::mbar_init(&x.response_full, 1);
+    if (tid == 17 || tid == 18) {
+      tc::mbar_init(&x.ticket_full[tid - 17], 1);
+      tc::mbar_init(&x.ticket_free[tid - 17], uint32_t(parts));
+    }
+    tc::fence_mbar_init();
+  }
+  __syncthreads();
+  if (parts > 1) {  // the barriers of every CTA of the cluster are set before one of them is arrived on
+    tc::cluster_arrive();
+    tc::cluster_wait();
+  }
+  bool ok = true;
+  QueueReader reader;
+  QueuedRow row;
+  Place buf(parts > 1 ? kBuf / 2 : kBuf), slot(kSlots);
+
+  if (warp < kRoleWarps) {
+    // ------------------------------------------------------------------------------------------- statistics
+    Place read(buf.size);  // half of the buffers behind buf
+    int ahead = 0;
+    while ((ok = ok && reader.next(x, row)) && row.row >= 0) {
+      if (row.label < 0) continue;
+      const RowShare<T> sh(logits + row.row * a.ld, V, per, rank);
+      Stats st{-INFINITY, 0.f, 0.f};
+      for (int at = 0; at < sh.count && ok; at += kChunk, slot.next()) {
+        ok = warp_wait(&x.full[slot.i], slot.parity);
+        const uint32_t src = ring + uint32_t(slot.i * kChunk + tid) * 16u;
+        const int left = sh.count - at - tid;
+        uint4 v[kPer];
+        if (left >= kChunk) {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) v[i] = lds16(src + i * kRoleThreads * 16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            v[i] = make_uint4(Vec<T>::kFill, Vec<T>::kFill, Vec<T>::kFill, Vec<T>::kFill);
+            if (i * kRoleThreads < left) v[i] = lds16(src + i * kRoleThreads * 16);
+          }
+        }
+        if (sh.ragged) {  // what lies outside the row becomes -inf
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int j0 = (sh.v0 + at + tid + i * kRoleThreads) * E - sh.off;
+            if (i * kRoleThreads < left && (j0 < 0 || j0 + E > V)) v[i] = mask_edge<T>(v[i], j0, V);
+          }
+        }
+        if (kGrad == 0) {  // nobody else reads the chunk
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&x.empty[slot.i]);
+        }
+        add_vectors<T, kPer, true>(st, v, a.k);
+      }
+      st = merge_warp<true>(st, a.k);
+      if (kGrad == 0 && ++ahead > buf.size / 2) {
+        ok = ok && warp_wait(&x.coef_full[read.i], read.parity);
+        read.next();
+      }
+      if (ok && lane < parts) {
+        const int to = (buf.i * parts + rank) * kRoleWarps + warp;
+        if (parts == 1) {
+          x.part[to] = make_float4(st.m, st.s, st.u, 0.f);
+          tc::mbar_arrive(&x.part_full[buf.i]);
+        } else {
+          st_async(&x.part[to], &x.part_full[buf.i], uint32_t(lane), st.m, st.s, st.u);
+        }
+      }
+      buf.next();
+    }
+  } else if (warp < 2 * kRoleWarps) {
+    // --------------------------------------------------------------------------------------------- gradient
+    // (without one its warps leave at once)
+    const int tg = tid - kRoleThreads;
+    const bool same = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.dlogits)) & 15) == 0 &&
+                      ((a.ld - a.ld_d) * int64_t(sizeof(T)) & 15) == 0;
+    while (kGrad != 0 && (ok = ok && reader.next(x, row)) && row.row >= 0) {
+      const RowShare<T> sh(logits + row.row * a.ld, V, per, rank);
+      T* dz = static_cast<T*>(a.dlogits) + row.row * a.ld_d;
+      const bool live = row.label >= 0, plain = same && !sh.ragged;
+      RowCoef o{0.f, 0.f, 0.f, 0.f, -1};
+      if (live) {
+        ok = warp_wait(&x.coef_full[buf.i], buf.parity);
+        o = x.coef[buf.i];
+        buf.next();
+      }
+      const int label = o.y < 0 ? -1 : (o.y + sh.off) / E - sh.v0;  // its vector of the share
+      for (int at = 0; at < sh.count && ok; at += kChunk) {
+        uint4 v[kPer];
+        if (live) {
+          ok = warp_wait(&x.full[slot.i], slot.parity);  // at once: the statistics role has read the chunk
+          const uint32_t src = ring + uint32_t(slot.i * kChunk + tg) * 16u;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) v[i] = lds16(src + i * kRoleThreads * 16);
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&x.empty[slot.i]);
+          slot.next();
+        }
+        const int left = sh.count - at - tg, j0 = (sh.v0 + at + tg) * E - sh.off;
+        if (plain && o.y >= 0) {
+          uint4* dst = reinterpret_cast<uint4*>(dz + j0);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            float2 g[E / 2];
+            vector_grad<T, kGrad>(v[i], o.m, a.k, o.A, o.B, g);
+            if (i * kRoleThreads < left) dst[i * kRoleThreads] = Vec<T>::pack(g);
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < kPer; ++i) {
+            if (i * kRoleThreads >= left) break;
+            const int ji = j0 + i * kRoleThreads * E;
+            float2 g[E / 2] = {};
+            const uint4 vi = i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3];
+            if (o.y >= 0) vector_grad<T, kGrad>(vi, o.m, a.k, o.A, o.B, g);
+            if (same && ji >= 0 && ji + E <= V)
+              *reinterpret_cast<uint4*>(dz + ji) = Vec<T>::pack(g);
+            else
+              store_edge<T>(dz, Vec<T>::pack(g), ji, V);
+          }
+        }
+        // the label's own entry, after its thread's store of the vector
+        if (label >= at && label < at + kChunk && label < sh.count && (label & (kRoleThreads - 1)) == tg)
+          from_f32(dz + o.y, o.at_label);
+      }
+    }
+  } else if (warp < 2 * kRoleWarps + kControlWarps) {
+    // ---------------------------------------------------------------------------------------------- control
+    const bool write = rank == 0 && lane == 0;
+    // The rows that count are taken in turn (so that one's buffer was last used by a row that this warp, too, has seen
+    // done: a wait by parity cannot tell that use from the one two before), and so are the others.
+    int turn = warp - 2 * kRoleWarps, dead_turn = turn;
+    while ((ok = ok && reader.next(x, row)) && row.row >= 0) {
+      int& next = row.label < 0 ? dead_turn : turn;
+      const bool mine = next == 0;
+      next = next == 0 ? kControlWarps - 1 : next - 1;
+      if (row.label < 0) {
+        if (!mine) continue;
+        if (lane == 0 && row.label == -2) record_device_error(&g_loss_error, kErrSlotOutOfRange);
+        if (write) finish_dead_row(a, t, row.row);
+        continue;
+      }
+      if (!mine) {
+        buf.next();
+        continue;
+      }
+      // asked for while the row's statistics are still being formed
+      const float zy = to_f32((logits + row.row * a.ld)[row.label]);
+      const PolicyIn in = policy_inputs(t, row.row);
+      ok = wait_cluster(&x.part_full[buf.i], buf.parity);
+      if (!ok) break;
+      if (parts > 1 && lane == 0) tc::mbar_arrive_expect_tx(&x.part_full[buf.i], part_bytes);  // for its next use
+      const Stats st = merge_parts<true>(x.part + buf.i * parts * kRoleWarps, parts * kRoleWarps, a.k);
+      const RowCoef o = finish_row<true, kGrad>(a, t, in, row.row, row.label, zy, st, write);
+      if (lane == 0) {
+        x.coef[buf.i] = o;
+        tc::mbar_arrive(&x.coef_full[buf.i]);
+      }
+      buf.next();
+    }
+  } else {
+    // --------------------------------------------------------------------------------------------- producer
+    Place q(kQueue), tk(2);
+    uint32_t response_parity = 0;
+    const auto push = [&](int64_t r, int label) {
+      if (q.wrapped) ok = ok && warp_wait(&x.queue_empty[q.i], q.parity ^ 1u);
+      if (lane == 0) {
+        x.queue[q.i] = QueuedRow{r, label, 0};
+        tc::mbar_arrive(&x.queue_full[q.i]);
+      }
+      q.next();
+    };
+    // Group k's rows are copied while the answer about group k + 2 is on its way: group k + 1's is read, and passed on
+    // to the cluster, before group k is begun.
+    int group = int(blockIdx.x) / parts, next = -1;
+    if (rank == 0 && lane == 0) request_rows(&x.response, &x.response_full);
+    while (ok && group >= 0) {
+      const int64_t first = int64_t(group) * group_rows;
+      const int rows = int(min(int64_t(group_rows), a.n - first));
+      int mine = -1;
+      if (lane < rows) {
+        const int64_t y = ld_index(a.labels, a.index_dtype, first + lane);
+        mine = y == a.ignore_index ? -1 : (y < 0 || y >= V) ? -2 : int(y);
+      }
+      if (rank == 0) {
+        const bool answered = warp_wait(&x.response_full, response_parity);
+        response_parity ^= 1u;
+        const int64_t cta = answered ? requested_cta(&x.response) : -1;
+        next = cta < 0 ? -1 : int(cta / parts);
+        ok = ok && answered;
+        tc::fence_proxy_async_smem();  // read before the next answer is written there
+        __syncwarp();
+        if (next >= 0 && lane == 0) request_rows(&x.response, &x.response_full);
+        if (parts > 1) {
+          if (tk.wrapped) ok = wait_cluster(&x.ticket_free[tk.i], tk.parity ^ 1u) && ok;
+          if (lane < parts) {
+            const uint32_t to = tc::mapa(tc::smem_u32(&x.ticket[tk.i]), uint32_t(lane));
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(next) : "memory");
+            arrive_cluster(&x.ticket_full[tk.i], uint32_t(lane));
+          }
+        }
+      }
+      for (int i = 0; i < rows && ok; ++i) {
+        const int64_t r = first + i;
+        const int label = __shfl_sync(0xffffffffu, mine, i);
+        push(r, label);
+        if (label < 0) continue;
+        const T* z = logits + r * a.ld;
+        const RowShare<T> sh(z, V, per, rank);
+        // a vector that reaches over an end of the row is copied whole, unless that end is the tensor's
+        const bool head = r == 0 && sh.v0 == 0 && sh.off > 0;
+        const bool tail = r == a.n - 1 && (sh.v0 + sh.count) * E - sh.off > V;
+        for (int at = 0; at < sh.count && ok; at += kChunk, slot.next()) {
+          if (slot.wrapped) ok = warp_wait(&x.empty[slot.i], slot.parity ^ 1u);
+          if (lane != 0 || !ok) continue;
+          const uint32_t dst = ring + uint32_t(slot.i * kChunk) * 16u;
+          int lo = at, hi = min(at + kChunk, sh.count);
+          if (head && lo == 0) {
+            sts16(dst, load_edge(z, -sh.off, V));
+            ++lo;
+          }
+          if (tail && hi == sh.count && hi > lo) {
+            --hi;
+            sts16(dst + (hi - at) * 16, load_edge(z, (sh.v0 + hi) * E - sh.off, V));
+          }
+          const uint32_t bytes = uint32_t(hi - lo) * 16u;
+          if (bytes) {
+            tc::mbar_arrive_expect_tx(&x.full[slot.i], bytes);
+            tc::bulk_load(dst + (lo - at) * 16, z + ((sh.v0 + lo) * E - sh.off), bytes, &x.full[slot.i]);
+          } else {
+            tc::mbar_arrive(&x.full[slot.i]);
+          }
+        }
+      }
+      if (parts > 1) {
+        ok = wait_cluster(&x.ticket_full[tk.i], tk.parity) && ok;
+        next = x.ticket[tk.i];
+        __syncwarp();
+        if (lane == 0) arrive_cluster(&x.ticket_free[tk.i], 0);
+        tk.next();
+      }
+      group = next;
+    }
+    if (!ok && rank == 0 && next >= 0)  // an answer is on its way: it lands before the CTA leaves
+      tc::mbar_wait_bounded(&x.response_full, response_parity, 1u << 16);
+    push(-1, -1);
+    if (!ok)  // copies in flight land before the CTA leaves: wait for every slot's last use
+      for (int i = 0; i < kSlots; ++i)
+        if (slot.wrapped || i < slot.i)
+          tc::mbar_wait_bounded(&x.full[i], i < slot.i ? slot.parity : slot.parity ^ 1u, 1u << 16);
+  }
+  if (!ok && lane == 0) record_device_error(&g_loss_error, kErrLossWaitTimeout);
+  if (parts > 1) {  // no CTA leaves while another may still write to its shared memory
+    tc::cluster_arrive();
+    tc::cluster_wait();
   }
 }
 
 // ------------------------------------------------------------------------------------------- distillation
-template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_kernel(LossRows a, DistillTerms t) {
+// Teacher entries are held in shared memory; a bit per element of the share marks the teacher's ids, so that the
+// student's mass outside them is a sum of its own (one minus the mass inside would lose what is left when that is
+// near one).  The gradient is written densely, then the entries at the ids are written over.
+template <typename T, int NT, bool kTail, bool kGrad>
+__global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, DistillTerms t, int parts) {
   extern __shared__ float sm[];
-  __shared__ float red[kThreads / 32];
-  float* tp = sm;                                 // [K] teacher probabilities
-  int* tid = reinterpret_cast<int*>(sm + t.K);    // [K] ids, -1 where there is none
-  const int64_t r = blockIdx.x;
-  const T* z = static_cast<const T*>(a.logits) + r * a.ld;
-  T* dz = a.dlogits ? static_cast<T*>(a.dlogits) + r * a.ld_d : nullptr;
-  const int V = int(a.V), K = t.K;
-  const float w = t.weights ? t.weights[r] : *t.scale;
-  // teacher: log p_k = t_k / T - its log-sum-exp (given, or over the entries of the row)
-  float tm = -INFINITY, valid = 0.f;
-  for (int k = threadIdx.x; k < K; k += kThreads) {
-    const int64_t id = ld_index(t.ids, a.index_dtype, r * K + k);
-    const bool ok = id >= 0 && id < V;
-    if (id >= V) record_device_error(&g_loss_error, kErrSlotOutOfRange);
-    tid[k] = ok ? int(id) : -1;
+  const int K = t.K;
+  float* tp = sm;                                // [K] teacher logits, then probabilities
+  int* id = reinterpret_cast<int*>(sm + K);      // [K] ids, -1 where there is none
+  __shared__ uint32_t mark[NT * kNV / 4];        // a byte per vector of a round, a bit per element
+  __shared__ float ts[2];                        // sum of p; log of the teacher's sum of exponentials
+  __shared__ int twice;                          // an id was given twice
+  const int64_t r = blockIdx.x / unsigned(parts);
+  const int rank = int(blockIdx.x % unsigned(parts));
+  const Share<T> w(a, r, rank, parts);
+  const int tid = int(threadIdx.x), lane = tid & 31;
+  const bool first = rank == 0 && tid == 0;
+  if (ld_index(t.ids, a.index_dtype, r * K) < 0) {  // the row counts for nothing (the same for the cluster)
+    if (first) t.divergence[r] = 0.f, t.row_loss[r] = 0.f;
+    if (kGrad) w.template zero<NT>(tid);
+    return;
+  }
+  if (parts > 1) tc::cluster_arrive();
+  uint4 v[kNV];
+  auto load = [&](int at) {
+#pragma unroll
+    for (int i = 0; i < kNV; ++i) {
+      const int vi = at + tid + i * NT;
+      v[i] = vi < w.v1 ? w.load(vi) : make_uint4(Vec<T>::kFill, Vec<T>::kFill, Vec<T>::kFill, Vec<T>::kFill);
+    }
+  };
+  load(w.v0);
+  if (tid == 0) twice = 0;
+  int valid = 0;
+  for (int k = tid; k < K; k += NT) {
+    const int64_t i = ld_index(t.ids, a.index_dtype, r * K + k);
+    const bool ok = i >= 0 && i < w.V;
+    if (i >= w.V) record_device_error(&g_loss_error, kErrSlotOutOfRange);
+    id[k] = ok ? int(i) : -1;
     tp[k] = ok ? ld_as_f32(t.logits, t.dtype, r * K + k) : -INFINITY;
-    tm = fmaxf(tm, tp[k]);
-    valid += ok ? 1.f : 0.f;
+    valid |= ok;
   }
-  tm = block_max(tm, red);
-  if (block_sum(valid, red) == 0.f || ld_index(t.ids, a.index_dtype, r * K) < 0) {  // the row counts for nothing
-    if (threadIdx.x == 0) t.divergence[r] = 0.f, t.row_loss[r] = 0.f;
-    if (dz) zero_row(dz, V);
-    return;
+  const bool any = __syncthreads_or(valid) != 0;
+  if (tid < 32) {  // the teacher's probabilities, by one warp while the others go on
+    float tm = -INFINITY, sum = 0.f, ps = 0.f;
+    if (!t.lse) {
+      for (int k = lane; k < K; k += 32) tm = fmaxf(tm, tp[k]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+      for (int k = lane; k < K; k += 32)
+        if (id[k] >= 0) sum += ex2((tp[k] - tm) * a.k);
+      sum = logf(warp_sum(sum));
+    }
+    for (int k = lane; k < K; k += 32) {
+      const float lp = t.lse ? fmaf(tp[k], a.inv_t, -t.lse[r]) : fmaf(tp[k] - tm, a.inv_t, -sum);
+      tp[k] = id[k] < 0 ? -INFINITY : lp;
+      if (id[k] >= 0) ps += expf(lp);
+    }
+    ps = warp_sum(ps);
+    if (lane == 0) ts[0] = ps;
   }
-  float tl = 0.f;  // log of the sum of the teacher's exponentials below its largest entry
-  if (!t.lse) {
-    for (int k = threadIdx.x; k < K; k += kThreads) tl += ex2((tp[k] - tm) * a.k);
-    tl = logf(block_sum(tl, red));
-  }
-  // student
-  float mx = -INFINITY;
-  for (int j = threadIdx.x; j < V; j += kThreads) mx = fmaxf(mx, to_f32(z[j]));
-  mx = block_max(mx, red);
-  float s = 0.f, rest = 0.f;  // all of the row, and what lies outside the teacher's ids
-  for (int j = threadIdx.x; j < V; j += kThreads) {
-    const float e = ex2((to_f32(z[j]) - mx) * a.k);
-    s += e;
-    if (t.lse) {
-      bool in = false;
-      for (int k = 0; k < K; ++k) in |= tid[k] == j;
-      if (!in) rest += e;
+  const int rounds = max(1, (w.v1 - w.v0 + NT * kNV - 1) / (NT * kNV));
+  Stats st{-INFINITY, 0.f, 0.f};  // s: outside the ids (kTail) or everywhere; u: at the ids (kTail)
+  for (int q = 0; q < rounds; ++q) {
+    const int at = w.v0 + q * NT * kNV;
+    if (q > 0) {
+      __syncthreads();
+      load(at);
+    }
+#pragma unroll
+    for (int i = 0; i < kNV / 4; ++i) mark[tid + i * NT] = 0u;
+    __syncthreads();
+    for (int k = tid; k < K; k += NT) {
+      if (id[k] < 0) continue;
+      const int vi = (id[k] + w.off) / Vec<T>::E - at;
+      if (vi < 0 || vi >= NT * kNV || vi + at >= w.v1) continue;
+      const uint32_t bit = 1u << (8 * (vi & 3) + (id[k] + w.off) % Vec<T>::E);
+      if (atomicOr(&mark[vi >> 2], bit) & bit) {
+        twice = 1;
+      } else if (kTail) {
+        const float zk = to_f32(w.z[id[k]]), m = fmaxf(st.m, zk);
+        rescale<false>(st, m, a.k);
+        st.u += zk == -INFINITY ? 0.f : ex2((zk - m) * a.k);
+      }
+    }
+    __syncthreads();
+    const float m = fmaxf(st.m, Vec<T>::template largest<kNV>(v));
+    rescale<false>(st, m, a.k);
+    const float b = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < kNV; ++i) {
+      float s, u;
+      if constexpr (kTail) {
+        const uint32_t bits = reinterpret_cast<const uint8_t*>(mark)[tid + i * NT];
+        if (bits != 0) {  // a few vectors of a row: element by element
+#pragma unroll
+          for (int e = 0; e < Vec<T>::E; ++e) {
+            const float2 z2 = Vec<T>::pair(v[i], e / 2);
+            const float x = ex2((((e & 1) ? z2.y : z2.x) - b) * a.k);
+            if (!(bits >> e & 1u)) st.s += x;
+          }
+          continue;
+        }
+      }
+      accumulate<T, 1, false>(v + i, b, a.k, s, u);
+      st.s += s;
     }
   }
-  s = block_sum(s, red);
-  rest = block_sum(rest, red);
-  const float l2s = log2f(s);
-  float kl = 0.f, ps = 0.f;
-  for (int k = threadIdx.x; k < K; k += kThreads) {
-    if (tid[k] < 0) {
-      tp[k] = 0.f;
-      continue;
+  if (parts > 1) tc::cluster_wait();
+  st = merge_rows<NT, false>(st, a.k, rank, parts);
+  const float S = kTail ? st.s + st.u : st.s, ls = logf(S), ps = ts[0];
+  // what is left of both; where the student has nothing left, a rest of the size of the sum's rounding is none
+  const float qr = kTail ? st.s / S : 1.f;
+  float pr = kTail ? fmaxf(1.f - ps, 0.f) : 0.f;
+  if (qr == 0.f && pr < 0x1p-20f) pr = 0.f;
+  const float wt = t.weights ? t.weights[r] : *t.scale;
+  if (rank == 0 && tid < 32) {
+    float kl = 0.f;
+    for (int k = lane; k < K; k += 32) {
+      const float lp = tp[k], p = expf(lp);
+      if (p != 0.f) kl = fmaf(p, lp - ((to_f32(w.z[id[k]]) - st.m) / a.temperature - ls), kl);
     }
-    const float lp = t.lse ? fmaf(tp[k], a.inv_t, -t.lse[r]) : fmaf(tp[k] - tm, a.inv_t, -tl);
-    const float p = expf(lp);
-    tp[k] = p;
-    ps += p;
-    if (p > 0.f) kl = fmaf(p, lp - kLn2 * ((to_f32(z[tid[k]]) - mx) * a.k - l2s), kl);
-  }
-  kl = block_sum(kl, red);
-  ps = block_sum(ps, red);
-  float A = ps, R = 0.f;
-  if (t.lse) {
-    const float pr = fmaxf(1.f - ps, 0.f), qr = rest / s;
+    kl = warp_sum(kl);
     if (pr > 0.f) kl += pr * (logf(pr) - logf(qr));
-    A = ps + pr;
-    R = pr > 0.f ? pr / qr : 0.f;
+    if (lane == 0) {
+      t.divergence[r] = any ? kl : 0.f;
+      t.row_loss[r] = any && wt != 0.f ? wt * t.t2 * kl : 0.f;
+    }
   }
-  if (threadIdx.x == 0) {
-    t.divergence[r] = kl;
-    t.row_loss[r] = w == 0.f ? 0.f : w * t.t2 * kl;
-  }
-  if (!dz) return;
-  if (w == 0.f) {
-    zero_row(dz, V);
-    return;
-  }
-  const float c = w * t.temperature;
-  for (int j = threadIdx.x; j < V; j += kThreads) {
-    float P = 0.f;
-    bool in = false;
-    for (int k = 0; k < K; ++k)
-      if (tid[k] == j) P += tp[k], in = true;
-    const float q = ex2((to_f32(z[j]) - mx) * a.k) / s;
-    from_f32(dz + j, c * (in ? fmaf(q, A, -P) : q * (A - R)));
+  if constexpr (kGrad) {
+    if (wt == 0.f || !any) {
+      w.template zero<NT>(tid);
+      return;
+    }
+    const float c = wt * a.temperature, A = ps + pr, R = pr > 0.f && qr != 0.f ? pr / qr : 0.f;
+    const float f = c * (A - R) / S;
+    for (int q = rounds - 1; q >= 0; --q) {
+      if (q < rounds - 1) load(w.v0 + q * NT * kNV);
+#pragma unroll
+      for (int i = 0; i < kNV; ++i) {
+        const int vi = w.v0 + q * NT * kNV + tid + i * NT;
+        if (vi >= w.v1) break;
+        float2 g[Vec<T>::E / 2];
+        vector_grad<T, 1>(v[i], st.m, a.k, f, 0.f, g);
+        w.store(vi, g);
+      }
+    }
+    __syncthreads();  // the dense gradient is written: the ids' entries go over it
+    for (int k = tid; k < K; k += NT) {
+      if (id[k] < 0) continue;
+      const int vi = (id[k] + w.off) / Vec<T>::E;
+      if (vi < w.v0 || vi >= w.v1) continue;
+      float P = expf(tp[k]);
+      if (twice) {  // every one of them writes the sum
+        P = 0.f;
+        for (int i = 0; i < K; ++i)
+          if (id[i] == id[k]) P += expf(tp[i]);
+      }
+      const float qk = ex2((to_f32(w.z[id[k]]) - st.m) * a.k) / S;
+      from_f32(w.dz + id[k], c * fmaf(qk, A, -P));
+    }
   }
 }
 
 // -------------------------------------------------------------------------------------------- small kernels
+constexpr int kSmall = 256;
+
+__device__ __forceinline__ double block_sum_f64(double v, double* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int w = 0; w < int(blockDim.x >> 5); ++w) v += red[w];
+  return v;
+}
+
 // scale = 1 / (rows that count): rows whose label is not ignore_index, or (K > 0) whose first id is >= 0
 __global__ void __launch_bounds__(1024) live_scale_kernel(const void* __restrict__ labels, int index_dtype, int64_t n,
                                                           int64_t stride, bool by_sign, int64_t ignore_index,
@@ -319,8 +1208,8 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* __restrict_
 
 // One CTA per pair (sequences 2p chosen, 2p + 1 rejected): the log ratios of both, the pair's loss, and
 // d loss / d logp of their tokens.
-__global__ void __launch_bounds__(kThreads) pair_kernel(PairTerms t) {
-  __shared__ double red[kThreads / 32];
+__global__ void __launch_bounds__(kSmall) pair_kernel(PairTerms t) {
+  __shared__ double red[kSmall / 32];
   const int64_t p = blockIdx.x;
   int64_t lo[2], hi[2];
   double sum[2], cnt[2];
@@ -332,7 +1221,7 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(PairTerms t) {
       lo[i] = hi[i] = 0;
     }
     double v = 0.0, c = 0.0;
-    for (int64_t r = lo[i] + threadIdx.x; r < hi[i]; r += kThreads) {
+    for (int64_t r = lo[i] + threadIdx.x; r < hi[i]; r += kSmall) {
       if (ld_index(t.labels, t.index_dtype, r) == t.ignore_index) continue;
       v += double(t.logps[r]) - (t.ref ? double(t.ref[r]) : 0.0);
       c += 1.0;
@@ -353,26 +1242,145 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(PairTerms t) {
   }
   for (int i = 0; i < 2; ++i) {
     const float c = float((i == 0 ? dh : -dh) * double(t.beta) / (double(t.pairs) * cnt[i]));
-    for (int64_t r = lo[i] + threadIdx.x; r < hi[i]; r += kThreads) t.coef[r] = c;
+    for (int64_t r = lo[i] + threadIdx.x; r < hi[i]; r += kSmall) t.coef[r] = c;
   }
 }
 
 // x *= *scale, row by row; nothing is read or written where the scale is one
 template <typename T>
-__global__ void __launch_bounds__(kThreads) scale_kernel(T* __restrict__ x, int64_t ld, int64_t n, int64_t V,
+__global__ void __launch_bounds__(kSmall) scale_kernel(T* __restrict__ x, int64_t ld, int64_t n, int64_t V,
                                                          const float* __restrict__ scale) {
   const float f = *scale;
   if (f == 1.f) return;
   for (int64_t r = blockIdx.x; r < n; r += gridDim.x)
-    for (int64_t j = threadIdx.x; j < V; j += kThreads) from_f32(x + r * ld + j, to_f32(x[r * ld + j]) * f);
+    for (int64_t j = threadIdx.x; j < V; j += kSmall) from_f32(x + r * ld + j, to_f32(x[r * ld + j]) * f);
+}
+
+// ------------------------------------------------------------------------------------------------- launches
+// How a row is split: threads of a CTA and CTAs of a row's cluster.
+struct Split {
+  int threads, parts;  // threads of a row's CTA (32: a warp of one with four rows), CTAs of a row's cluster
+};
+
+// the most 16-byte vectors that a row reaches into
+int64_t row_vectors(const LossRows& a) {
+  const int64_t E = a.dtype == KDN_DTYPE_BF16 ? 8 : 4;
+  const bool aligned = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && (a.ld % E == 0 || a.n == 1);
+  return aligned ? (a.V + E - 1) / E : (a.V + 2 * E - 2) / E;
+}
+
+// Kernels that keep a row's share in registers.  Many short rows: a warp each (B200, policy loss with gradient, bf16,
+// 16384 x 1000: 27 us against 74 with 128 threads a row; 16384 x 4096: 65 against 92, but 600 x 4096: 10.8 against
+// 9.1).  Else enough threads to hold the row, over more CTAs where one is too small, but (few rows being spread over
+// the SMs at best) no more than two CTAs an SM.
+Split choose_split(const LossRows& a) {
+  const int64_t vecs = row_vectors(a), sms = current_sm_count();
+  if ((vecs <= 256 && a.n >= 2 * sms) || (vecs <= 512 && a.n >= 8 * sms)) return Split{32, 1};
+  Split s{vecs <= 128 * kNV ? 128 : vecs <= 256 * kNV ? 256 : 512, 1};
+  while (s.parts < kMaxCluster && vecs > int64_t(s.threads) * kNV * s.parts && a.n * s.parts < 2 * sms) s.parts *= 2;
+  return s;
+}
+
+// Log-probabilities alone read a row once and keep nothing of it: where there are rows enough, small CTAs in as many
+// rounds as it takes (at different places of their rows, those of an SM keep the memory busy).  B200, bf16: 16384 x 4096
+// 26 us with a warp a row, 53 with 128 threads; 4096 x 32000 47 us with 128 threads, 65 with the row in the registers of
+// 512; 2400 x 131072 101 us with 256 threads, 107 with 128, 326 with a cluster of four times 512.
+Split choose_scan_split(const LossRows& a) {
+  if (a.n < 2 * current_sm_count()) return choose_split(a);
+  const int64_t vecs = row_vectors(a);
+  return Split{vecs <= 1024 ? 32 : vecs <= 8192 ? 128 : 256, 1};
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch_rows(void (*kernel)(KArgs...), int64_t rows, Split s, bool cluster, size_t smem,
+                        cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  if (s.threads == 32) rows = (rows + 3) / 4, s.threads = 128;
+  cfg.gridDim = dim3(unsigned(rows * s.parts));
+  cfg.blockDim = dim3(unsigned(s.threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = unsigned(s.parts);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = cluster && s.parts > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args..., s.parts);
+}
+
+// f(T of the logits, threads) as types
+template <typename F>
+cudaError_t dispatch(const LossRows& a, Split s, F f) {
+  using std::integral_constant;
+  if (a.dtype == KDN_DTYPE_BF16) {
+    if (s.threads == 32) return f(__nv_bfloat16{}, integral_constant<int, 32>{});
+    if (s.threads == 128) return f(__nv_bfloat16{}, integral_constant<int, 128>{});
+    if (s.threads == 256) return f(__nv_bfloat16{}, integral_constant<int, 256>{});
+    return f(__nv_bfloat16{}, integral_constant<int, 512>{});
+  }
+  if (s.threads == 32) return f(float{}, integral_constant<int, 32>{});
+  if (s.threads == 128) return f(float{}, integral_constant<int, 128>{});
+  if (s.threads == 256) return f(float{}, integral_constant<int, 256>{});
+  return f(float{}, integral_constant<int, 512>{});
+}
+
+// The CTAs of a row's cluster and the vectors of each one's share in the streaming kernel; parts = 0: the rows are too
+// long for its ring, which has to hold a row's share and what is being copied of the next one's, or it does not pay:
+// rows of up to 32 KiB, or fewer than two an SM.  Measured on B200, policy loss with gradient, bf16, streaming kernel
+// against CTAs that keep a row in registers: 2400 x 4096 30.3 us against 18.8, 148 x 32000 11.5 against 9.4, 600 x
+// 32000 26.8 against 26.1, 2400 x 32000 69.4 against 77.2, 2400 x 131072 236 against 330.  The choice does not depend
+// on whether a gradient is asked for, so that the outputs do not either.
+struct Stream {
+  int parts, per;
+};
+Stream choose_stream(const LossRows& a) {
+  const int64_t vecs = row_vectors(a);
+  if (vecs <= 2048 || a.n < 2 * current_sm_count()) return {0, 0};
+  for (int parts = 1; parts <= kMaxCluster; parts *= 2) {
+    const int64_t per = (vecs + parts - 1) / parts;
+    if (per <= 9 * kChunk) return {parts, int(per)};
+  }
+  return {0, 0};
+}
+
+// Rows of one request: as many as make 128 KiB, as long as that leaves every SM eight requests to even out what ignored
+// rows save.
+int64_t group_rows(const LossRows& a, Stream s) {
+  const int64_t chunks = (s.per + kChunk - 1) / kChunk, most = a.n * s.parts / (8 * current_sm_count());
+  return std::max<int64_t>(1, std::min<int64_t>(8 / chunks, most));
+}
+
+template <typename K>
+cudaError_t launch_stream(K kernel, const LossRows& a, const PolicyTerms& t, Stream s, cudaStream_t stream) {
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRingBytes));
+      e != cudaSuccess)
+    return e;
+  const int64_t group = group_rows(a, s);
+  return launch_rows(kernel, (a.n + group - 1) / group, Split{kStreamThreads, s.parts}, true, kRingBytes, stream, a, t,
+                     int(group), s.per);
 }
 
 cudaError_t launch_logp(const LossRows& a, const PolicyTerms& t, cudaStream_t stream) {
-  if (a.dtype == KDN_DTYPE_BF16)
-    logp_kernel<__nv_bfloat16><<<unsigned(a.n), kThreads, 0, stream>>>(a, t);
-  else
-    logp_kernel<float><<<unsigned(a.n), kThreads, 0, stream>>>(a, t);
-  return cudaGetLastError();
+  const Stream st = t.row_loss ? choose_stream(a) : Stream{0, 0};
+  if (st.parts > 0) {
+    const auto go = [&](auto z) {
+      using T = decltype(z);
+      if (!a.dlogits) return launch_stream(policy_stream_kernel<T, 0>, a, t, st, stream);
+      return t.entropy_coef != 0.f ? launch_stream(policy_stream_kernel<T, 2>, a, t, st, stream)
+                                   : launch_stream(policy_stream_kernel<T, 1>, a, t, st, stream);
+    };
+    return a.dtype == KDN_DTYPE_BF16 ? go(__nv_bfloat16{}) : go(float{});
+  }
+  const Split s = t.row_loss ? choose_split(a) : choose_scan_split(a);
+  return dispatch(a, s, [&](auto z, auto nt) {
+    using T = decltype(z);
+    constexpr int NT = decltype(nt)::value;
+    const auto go = [&](auto kernel) { return launch_rows(kernel, a.n, s, true, 0, stream, a, t); };
+    if (!t.row_loss) return go(logp_kernel<T, NT, false, 0>);
+    if (!a.dlogits) return go(logp_kernel<T, NT, true, 0>);
+    return t.entropy_coef != 0.f ? go(logp_kernel<T, NT, true, 2>) : go(logp_kernel<T, NT, true, 1>);
+  });
 }
 
 }  // namespace
@@ -382,11 +1390,14 @@ cudaError_t launch_token_logprobs(const LossRows& a, cudaStream_t stream) {
 }
 
 cudaError_t launch_token_logprobs_backward(const LossRows& a, const float* dlogps, cudaStream_t stream) {
-  if (a.dtype == KDN_DTYPE_BF16)
-    logp_backward_kernel<__nv_bfloat16><<<unsigned(a.n), kThreads, 0, stream>>>(a, dlogps);
-  else
-    logp_backward_kernel<float><<<unsigned(a.n), kThreads, 0, stream>>>(a, dlogps);
-  return cudaGetLastError();
+  // Nothing ties a row's CTAs together: at most two rounds of 256 threads each.  B200, bf16, 8192 x 32000: 165 us with
+  // 256 threads and one CTA a row, 180 with two CTAs, 173 with four of 128 threads, 190 with 512 threads and 4 vectors.
+  const int64_t vecs = row_vectors(a);
+  Split s{vecs <= 512 ? 32 : vecs <= 128 * kNV ? 128 : 256, 1};
+  while (vecs > 4096 * int64_t(s.parts)) s.parts *= 2;
+  return dispatch(a, s, [&](auto z, auto nt) {
+    return launch_rows(logp_backward_kernel<decltype(z), decltype(nt)::value>, a.n, s, false, 0, stream, a, dlogps);
+  });
 }
 
 cudaError_t launch_policy_loss(const LossRows& a, const PolicyTerms& t, float* loss, cudaStream_t stream) {
@@ -407,7 +1418,7 @@ cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, float*
     f.coef_zero = t.coef;
     if (cudaError_t e = launch_logp(f, PolicyTerms{}, stream); e != cudaSuccess) return e;
   }
-  pair_kernel<<<unsigned(t.pairs), kThreads, 0, stream>>>(t);
+  pair_kernel<<<unsigned(t.pairs), kSmall, 0, stream>>>(t);
   if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   loss_sum_kernel<<<1, 1024, 0, stream>>>(t.pair_loss, t.pairs, 1.0 / double(t.pairs), loss);
   if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
@@ -419,12 +1430,16 @@ cudaError_t launch_distillation_loss(const LossRows& a, const DistillTerms& t, f
     live_scale_kernel<<<1, 1024, 0, stream>>>(t.ids, a.index_dtype, a.n, t.K, true, 0, const_cast<float*>(t.scale));
     if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   }
-  const size_t smem = size_t(t.K) * 8;
-  if (a.dtype == KDN_DTYPE_BF16)
-    distill_kernel<__nv_bfloat16><<<unsigned(a.n), kThreads, smem, stream>>>(a, t);
-  else
-    distill_kernel<float><<<unsigned(a.n), kThreads, smem, stream>>>(a, t);
-  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+  Split s = choose_split(a);
+  s.threads = std::max(s.threads, 128);
+  const cudaError_t e = dispatch(a, s, [&](auto z, auto nt) {
+    using T = decltype(z);
+    constexpr int NT = decltype(nt)::value < 128 ? 128 : decltype(nt)::value;
+    const auto go = [&](auto kernel) { return launch_rows(kernel, a.n, s, true, size_t(t.K) * 8, stream, a, t); };
+    if (t.lse) return a.dlogits ? go(distill_kernel<T, NT, true, true>) : go(distill_kernel<T, NT, true, false>);
+    return a.dlogits ? go(distill_kernel<T, NT, false, true>) : go(distill_kernel<T, NT, false, false>);
+  });
+  if (e != cudaSuccess) return e;
   loss_sum_kernel<<<1, 1024, 0, stream>>>(t.row_loss, a.n, 1.0, loss);
   return cudaGetLastError();
 }
@@ -433,9 +1448,9 @@ cudaError_t launch_scale_rows(void* x, int dtype, int64_t ld, int64_t n, int64_t
                               cudaStream_t stream) {
   const unsigned grid = unsigned(n < 148 * 8 ? n : 148 * 8);
   if (dtype == KDN_DTYPE_BF16)
-    scale_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(static_cast<__nv_bfloat16*>(x), ld, n, V, scale);
+    scale_kernel<__nv_bfloat16><<<grid, kSmall, 0, stream>>>(static_cast<__nv_bfloat16*>(x), ld, n, V, scale);
   else
-    scale_kernel<float><<<grid, kThreads, 0, stream>>>(static_cast<float*>(x), ld, n, V, scale);
+    scale_kernel<float><<<grid, kSmall, 0, stream>>>(static_cast<float*>(x), ld, n, V, scale);
   return cudaGetLastError();
 }
 

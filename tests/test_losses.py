@@ -230,7 +230,9 @@ def test_token_logprobs_leading_dims_and_streams():
     y = torch.randint(0, 333, (2, 5), generator=g, device="cuda")
     flat = kdn.token_logprobs(z.view(10, 333), y.view(10))
     assert torch.equal(kdn.token_logprobs(z, y), flat.view(2, 5))
-    assert torch.equal(kdn.token_logprobs(z.transpose(0, 1), y.t()), flat.view(2, 5).t())  # rows of another order
+    # rows of another order lie elsewhere within 16 bytes (V is odd): sums in another order, within eps
+    other = kdn.token_logprobs(z.transpose(0, 1), y.t())
+    assert float((other - flat.view(2, 5).t()).abs().max()) <= 2 * _eps(z.view(10, 333), 1.0)
     assert torch.equal(kdn.token_logprobs(z[0].t().contiguous().t(), y[0]), flat[:5])      # columns not adjacent
     wide = torch.stack([y.view(10), y.view(10)], 1)[:, 0]                                   # strided labels
     assert torch.equal(kdn.token_logprobs(z.view(10, 333), wide), flat)
