@@ -894,7 +894,7 @@ int kdn_token_logprobs_backward(const void* logits, int dtype, int64_t ld, const
     return fail(KDN_ERR_INVALID, "labels/row_stats/dlogps/dlogits is NULL");
   kdn::LossRows a = loss_rows(logits, dtype, ld, labels, index_dtype, ignore_index, dlogits, ld_d, n, V, temperature);
   a.stats = const_cast<float*>(row_stats);
-  cudaError_t e = kdn::launch_token_logprobs_backward(a, dlogps, static_cast<cudaStream_t>(stream));
+  cudaError_t e = kdn::launch_token_logprobs_backward(a, dlogps, false, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "token log-probability backward launch");
   return ok();
 }

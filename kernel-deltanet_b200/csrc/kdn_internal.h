@@ -236,7 +236,8 @@ struct DistillTerms {
   float* divergence;      // [n]
 };
 cudaError_t launch_token_logprobs(const LossRows& a, cudaStream_t stream);
-cudaError_t launch_token_logprobs_backward(const LossRows& a, const float* dlogps, cudaStream_t stream);
+// `after`: the previous launch on the stream is of the same call
+cudaError_t launch_token_logprobs_backward(const LossRows& a, const float* dlogps, bool after, cudaStream_t stream);
 cudaError_t launch_policy_loss(const LossRows& a, const PolicyTerms& t, float* loss, cudaStream_t stream);
 cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, float* loss, cudaStream_t stream);
 cudaError_t launch_distillation_loss(const LossRows& a, const DistillTerms& t, float* loss, cudaStream_t stream);

@@ -16,7 +16,7 @@
 // passes over it (statistics, then gradient), so the logits are read from memory once and the gradient is written once;
 // the row's statistics are merged through warp shuffles, one barrier, and (in a cluster) one exchange through
 // distributed shared memory.  Longer shares are taken in rounds and read again for the gradient.  The second, for the
-// losses with a gradient over many long rows, streams them through a ring in shared memory: policy_stream_kernel.
+// losses with a gradient over many long rows, streams them through a ring in shared memory: loss_stream_kernel.
 #include <math.h>
 
 #include <algorithm>
@@ -74,6 +74,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "=f"(r.x), "=f"(r.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
+}
+
+// First thing in the kernels of a call that makes several launches: the next kernel of the same call may be launched (it waits in turn, its launch
+// overlaps this one's end), and the previous one's results are awaited (at once where it was launched without overlap).
+__device__ __forceinline__ void await_previous() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -292,14 +299,14 @@ __device__ __forceinline__ Stats merge_warp(Stats a, float k) {
   return a;
 }
 
-// ... of `count` <= 64 parts in shared memory, by every warp that asks
+// ... of `count` parts in shared memory, by every warp that asks
 template <bool kMoment>
 __device__ __forceinline__ Stats merge_parts(const float4* p, int count, float k) {
   const int lane = threadIdx.x & 31;
-  const float4 t = lane < count ? p[lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-  Stats a{t.x, t.y, t.z};
-  if (count > 32 && lane + 32 < count) {
-    Stats b{p[lane + 32].x, p[lane + 32].y, p[lane + 32].z};
+  Stats a{-INFINITY, 0.f, 0.f};
+  for (int i = lane; i < count; i += 32) {
+    const float4 t = p[i];
+    Stats b{t.x, t.y, t.z};
     const float m = fmaxf(a.m, b.m);
     rescale<kMoment>(a, m, k);
     rescale<kMoment>(b, m, k);
@@ -375,10 +382,12 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, const Poli
   return p;
 }
 
-// What the gradient of a row needs: dz_j = 2^d (A + B d) with d = (z_j - m) k, and dz_y.
+// What the gradient of a row needs: dz_j = 2^d (A + B d) with d = (z_j - m) k, and dz_y; for the distillation loss the
+// entries at the teacher's ids are c (total q - p), q = 2^d / sum.
 struct RowCoef {
   float m, A, B, at_label;
   int y;  // -1: the gradient is zero
+  float c, total, sum;
 };
 
 // From a row's statistics: its outputs (written where `write` is set) and the coefficients of its gradient.
@@ -396,7 +405,7 @@ __device__ __forceinline__ RowCoef finish_row(const LossRows& a, const PolicyTer
     if (a.stats) a.stats[2 * r] = st.m, a.stats[2 * r + 1] = st.s;
     if (a.coef_zero) a.coef_zero[r] = 0.f;
   }
-  RowCoef o{st.m, 0.f, 0.f, 0.f, -1};
+  RowCoef o{st.m, 0.f, 0.f, 0.f, -1, 0.f, 0.f, 0.f};
   if (!t.row_loss) return o;
   const float H = kEntropy ? fmaf(-kLn2, st.u / st.s, ls) : 0.f;
   const PolicyRow p = policy_row(t, in, logp, H);
@@ -420,6 +429,93 @@ __device__ __forceinline__ void finish_dead_row(const LossRows& a, const PolicyT
   if (a.coef_zero) a.coef_zero[r] = 0.f;
   if (t.entropy) t.entropy[r] = 0.f;
   if (t.row_loss) t.row_loss[r] = 0.f;
+}
+
+__device__ __forceinline__ void finish_dead_row(const LossRows&, const DistillTerms& t, int64_t r) {
+  t.divergence[r] = 0.f;
+  t.row_loss[r] = 0.f;
+}
+
+// p (log p - log q) of one teacher entry, added to kl; an entry of probability zero adds nothing
+__device__ __forceinline__ float distill_term(float kl, float lp, float z, float m, float temperature, float ls) {
+  const float p = expf(lp);
+  return p != 0.f ? fmaf(p, lp - ((z - m) / temperature - ls), kl) : kl;
+}
+
+// the teacher's probability at an id that is given more than once
+__device__ __forceinline__ float mass_at(const int* ids, const float* lp, int K, int id) {
+  float p = 0.f;
+  for (int k = 0; k < K; ++k)
+    if (ids[k] == id) p += expf(lp[k]);
+  return p;
+}
+
+// From the student's mass outside the ids (st.s) and at them (st.u), the teacher's mass at them (-1: it has no id) and
+// the divergence over them: the row's outputs and the coefficients of its gradient.  With P = sum p and, where the rest is
+// a class of its own, p_r = 1 - P and q_r the student's rest,
+//   dz_j = w T ((P + p_r) q_j - p_j) at an id,   w T (P + p_r - p_r / q_r) q_j elsewhere.
+// Where the student has nothing left, a rest of the size of the sum's rounding is none.
+__device__ __forceinline__ RowCoef finish_distill_row(const LossRows& a, const DistillTerms& t, int64_t r, float mass,
+                                                      float weight, float kl, const Stats& st, bool write) {
+  RowCoef o{st.m, 0.f, 0.f, 0.f, -1, 0.f, 0.f, 0.f};
+  o.sum = st.s + st.u;
+  const float qr = st.s / o.sum;
+  float pr = t.lse ? fmaxf(1.f - mass, 0.f) : 0.f;
+  if (qr == 0.f && pr < 0x1p-20f) pr = 0.f;
+  if (pr > 0.f) kl += pr * (logf(pr) - logf(qr));
+  if (write) {
+    t.divergence[r] = mass < 0.f ? 0.f : kl;
+    t.row_loss[r] = mass < 0.f || weight == 0.f ? 0.f : weight * t.t2 * kl;
+  }
+  if (mass < 0.f || weight == 0.f) return o;
+  o.y = 0;
+  o.c = weight * a.temperature;
+  o.total = mass + pr;
+  o.A = o.c * (o.total - (pr > 0.f && qr != 0.f ? pr / qr : 0.f)) / o.sum;
+  return o;
+}
+
+// One warp: a row's teacher entries (K <= 32 N), lane + 32 i a lane: ids (-1: none) and log-probabilities; returns the sum
+// of the probabilities, -1 without an id.
+template <int N>
+__device__ __forceinline__ float teacher_probabilities(const LossRows& a, const DistillTerms& t, int64_t r, bool record,
+                                                       int (&id)[N], float (&lp)[N]) {
+  const int lane = threadIdx.x & 31;
+  float m = -INFINITY, s = 0.f, mass = 0.f;
+  bool any = false;
+  int64_t j[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {  // all loads before the first use
+    const int k = lane + 32 * i;
+    j[i] = k < t.K ? ld_index(t.ids, a.index_dtype, r * t.K + k) : -1;
+    lp[i] = k < t.K ? ld_as_f32(t.logits, t.dtype, r * t.K + k) : -INFINITY;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (j[i] >= a.V) {
+      if (record) record_device_error(&g_loss_error, kErrSlotOutOfRange);
+      j[i] = -1;
+    }
+    id[i] = j[i] < 0 ? -1 : int(j[i]);
+    if (id[i] < 0) lp[i] = -INFINITY;
+    any |= id[i] >= 0;
+    m = fmaxf(m, lp[i]);
+  }
+  const float lse = t.lse ? t.lse[r] : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (id[i] >= 0) s += ex2((lp[i] - m) * a.k);
+  s = logf(warp_sum(s));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (id[i] < 0) continue;
+    lp[i] = t.lse ? fmaf(lp[i], a.inv_t, -lse) : fmaf(lp[i] - m, a.inv_t, -s);
+    mass += expf(lp[i]);
+  }
+  mass = warp_sum(mass);
+  return __any_sync(0xffffffffu, any) ? mass : -1.f;
 }
 
 // the gradient of one vector of logits (but for the label's own term)
@@ -481,6 +577,7 @@ __device__ __forceinline__ void add_vectors(Stats& st, const uint4* v, float k) 
 template <typename T, int NT, bool kEntropy, int kGrad>
 __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
     logp_kernel(LossRows a, PolicyTerms t, int parts) {
+  await_previous();
   const int64_t r = Cta<NT>::row(parts);
   if (r >= a.n) return;
   const int rank = int(blockIdx.x % unsigned(parts));
@@ -537,7 +634,8 @@ __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
 // d/dz of sum_t dlogps_t logp_t from the saved statistics: one read, one write, nothing to reduce
 template <typename T, int NT>
 __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
-    logp_backward_kernel(LossRows a, const float* __restrict__ dlogps, int parts) {
+    logp_backward_kernel(LossRows a, const float* dlogps, int parts) {
+  await_previous();
   const int64_t r = Cta<NT>::row(parts);
   if (r >= a.n) return;
   const int tid = int(threadIdx.x) % NT;
@@ -575,25 +673,41 @@ __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
 //   producer   takes the next group of rows (the grid has a cluster for each; a resident one cancels the launch of
 //              one that has not started and does its work instead, so SMs that met many ignored rows take more),
 //              reads their labels, queues them for the other roles, and copies the share of those that count into a
-//              ring of chunks in shared memory;
-//   statistics (8 warps) maximum and sums of every chunk as it arrives, then one partial result a warp;
-//              (in a cluster, to the shared memory of every CTA of it);
+//              ring of 16 KiB chunks in shared memory;
+//   teacher    (distillation only) forms the teacher's probabilities of a row;
+//   marker     (distillation only) adds up the exponentials at the teacher's ids in every chunk that arrives and puts
+//              -inf in their place, so that what the statistics role sums is the student's mass outside the ids (one
+//              minus the mass inside would lose it when that is near one);
+//   statistics (8 warps) maximum and sums of every chunk as it arrives, then one partial result a warp (in a cluster,
+//              to the shared memory of every CTA of it);
 //   control    (2 warps, row about) merges a row's partials, computes the loss, writes the row's outputs and
 //              publishes the coefficients of its gradient;
-//   gradient   (8 warps) reads the row's chunks once more from shared memory, writes the gradient, frees them.
-// Every wait is bounded; after one that gave up a role ends, kErrLossWaitTimeout is recorded, and the CTA returns
-// when its copies have landed.
+//   gradient   (8 warps) reads the row's chunks once more from shared memory, writes the gradient, frees them;
+//   patcher    (distillation only) writes the gradient's entries at the ids once the row's gradient is written.
+// A slot's, a row's and a buffer's barriers are waited for by each role at every use and in order: a wait by parity
+// cannot tell a use from the one two before.  Every wait is bounded; after one that gave up a role ends,
+// kErrLossWaitTimeout is recorded, and the CTA returns when its copies have landed.
 constexpr int kPer = 4;                // vectors that a thread of a role takes at a time
 constexpr int kBuf = 16;               // rows between a partial result and its use (8 in a cluster), see Exchange
 constexpr int kQueue = 32;             // rows between the producer and the last of the other roles
 constexpr int kRoleThreads = 256;      // of the statistics and of the gradient role
 constexpr int kRoleWarps = kRoleThreads / 32;
 constexpr int kControlWarps = 2;
-constexpr int kStreamThreads = 2 * kRoleThreads + 32 * (kControlWarps + 1);
+constexpr int kMaxTop = 128;           // teacher entries of a row that the streaming kernel takes
+constexpr int kTeachers = 6;           // rows between the teacher and the patcher (even: control takes rows in turn)
 constexpr uint32_t kLossWaitLimit = 1u << 20;
 constexpr int kChunk = kPer * kRoleThreads;  // vectors: 16 KiB
+
 constexpr int kSlots = 13;                   // chunks of the ring
 constexpr size_t kRingBytes = size_t(kSlots) * kChunk * 16;
+
+// What the kinds of losses differ in: their roles.
+template <typename Terms>
+struct Streaming {
+  static constexpr bool kDistill = std::is_same_v<Terms, DistillTerms>;
+  static constexpr int kParts = kRoleWarps + (kDistill ? 1 : 0);  // partial results of a row in a CTA
+  static constexpr int kThreads = 2 * kRoleThreads + 32 * (kControlWarps + 1 + (kDistill ? 3 : 0));
+};
 
 struct __align__(16) QueuedRow {
   int64_t row;  // -1: no more rows
@@ -601,19 +715,33 @@ struct __align__(16) QueuedRow {
   int pad;
 };
 
+// A row's teacher: log-probabilities at its ids (-1: none).
+struct Teacher {
+  float lp[kMaxTop];
+  int id[kMaxTop];
+};
+
 // What the roles pass on.  Rows that count use the buffers for partial results and coefficients in turn, 16 of them,
 // or 8 in a cluster.  They are free when they are written: with a gradient, the ring holds 13 rows at most (3 in a
 // cluster, where a share is more than 4 chunks), a row leaves it when its coefficients have been used, and another
-// CTA's control is at most that far behind its statistics; without, statistics wait for the control warps to be at
-// most half of the buffers behind.
+// CTA's control is at most that far behind its statistics; without, statistics (and the marker) wait for the control
+// warps to be at most half of the buffers behind.  The teachers' buffers are handed back by a barrier.
+template <bool kDistill>
 struct Exchange {
-  uint4 response;                                      // of a request for more rows
-  float4 part[kBuf / 2 * kRoleWarps * kMaxCluster];    // (m, s, u) of each statistics warp of the cluster
+  uint4 response;                                                  // of a request for more rows
+  float4 part[kBuf / 2 * kMaxCluster * (kRoleWarps + kDistill)];   // (m, s, u) of each statistics warp of the cluster
   QueuedRow queue[kQueue];
   RowCoef coef[kBuf];
-  int ticket[2];                         // the cluster's next group of rows, -1: none
-  uint64_t full[kSlots], empty[kSlots];
+  Teacher teacher[kDistill ? kTeachers : 1];
+  float mass[kTeachers];  // the sum of a teacher's probabilities, -1 without an id
+  int twice[kTeachers];   // an id was given twice
+  int ticket[2];          // the cluster's next group of rows, -1: none
+  uint32_t sink[2 * kRoleWarps];  // see free_chunk
+  uint32_t spare[32];
+  uint64_t full[kSlots], empty[kSlots], marked[kSlots];
   uint64_t part_full[kBuf], coef_full[kBuf];
+  uint64_t teacher_full[kTeachers], teacher_free[kTeachers];
+  uint64_t row_done[kTeachers];  // the gradient is written and the row's ids are known to be given once or more
   uint64_t queue_full[kQueue], queue_empty[kQueue];
   uint64_t response_full, ticket_full[2], ticket_free[2];
 };
@@ -708,51 +836,104 @@ struct RowShare {
   }
 };
 
+// Hands a chunk back once the warp's loads of it have returned.  An arrival does not wait for loads that are still under
+// way (it overtook them: the next copy was then read in their place); the store of a word that needs all of them does.
+template <int N>
+__device__ __forceinline__ void free_chunk(uint64_t* bar, const uint4 (&v)[N], uint32_t* sink) {
+  uint32_t all = 0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) all ^= v[i].x;
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(tc::smem_u32(sink)), "r"(all) : "memory");
+    tc::mbar_arrive(bar);
+  }
+}
+
 // The next row of a role's walk through the queue.
 struct QueueReader {
   Place at{kQueue};
-  __device__ __forceinline__ bool next(Exchange& x, QueuedRow& row) {
+  template <typename X>
+  __device__ __forceinline__ bool next(X& x, QueuedRow& row) {
     const bool ok = warp_wait(&x.queue_full[at.i], at.parity);
     if (ok) row = x.queue[at.i];
-    __syncwarp();
+    // through a shuffle: it needs the loaded values, and the slot is handed back after it
+    row.row = __shfl_sync(0xffffffffu, row.row, 0);
+    row.label = __shfl_sync(0xffffffffu, row.label, 0);
     if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&x.queue_empty[at.i]);
     at.next();
     return ok;
   }
 };
 
-template <typename T, int kGrad>
-__global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRows a, PolicyTerms t, int group_rows,
-                                                                        int per, int parts) {
+// Sets an element of a chunk in shared memory / reads it.
+template <typename T>
+__device__ __forceinline__ void put_bits(uint32_t a, uint32_t bits) {
+  if constexpr (sizeof(T) == 4)
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(bits) : "memory");
+  else
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(uint16_t(bits)) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ uint32_t get_bits(uint32_t a) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+  } else {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+    return v;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float bits_to_f32(uint32_t bits) {
+  return __uint_as_float(sizeof(T) == 4 ? bits : bits << 16);
+}
+
+template <typename T, typename Terms, int kGrad>
+__global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
+    loss_stream_kernel(LossRows a, Terms t, int group_rows, int per, int parts) {
   extern __shared__ __align__(128) uint8_t ring_mem[];
-  __shared__ Exchange x;
-  constexpr int E = Vec<T>::E;
+  constexpr bool kDistill = Streaming<Terms>::kDistill;
+  constexpr int E = Vec<T>::E, kParts = Streaming<Terms>::kParts;
+  // warps: statistics, gradient, control, producer, teacher, marker, patcher
+  constexpr int kGradWarp = kRoleWarps, kControlWarp = 2 * kRoleWarps, kProducerWarp = kControlWarp + kControlWarps;
+  constexpr int kTeacherWarp = kProducerWarp + 1, kMarkerWarp = kProducerWarp + 2;
+  __shared__ Exchange<kDistill> x;
   const int tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int rank = int(blockIdx.x % unsigned(parts)), V = int(a.V);
   const uint32_t ring = tc::smem_u32(ring_mem);
   const T* logits = static_cast<const T*>(a.logits);
-  const uint32_t part_bytes = uint32_t(kRoleWarps * parts) * 16u;
+  const uint32_t part_bytes = uint32_t(kParts * parts) * 16u;
   if (tid < 64) {  // a few barriers a thread
     if (tid < kSlots) {
       tc::mbar_init(&x.full[tid], 1);
       tc::mbar_init(&x.empty[tid], kRoleWarps);
+      tc::mbar_init(&x.marked[tid], 1);
     }
     if (tid < kBuf) {
-      tc::mbar_init(&x.part_full[tid], parts == 1 ? kRoleWarps : 1);
+      tc::mbar_init(&x.part_full[tid], parts == 1 ? kParts : 1);
       if (parts > 1) tc::mbar_arrive_expect_tx(&x.part_full[tid], part_bytes);
       tc::mbar_init(&x.coef_full[tid], 1);
     }
+    if (tid >= 16 && tid < 16 + kTeachers) {
+      tc::mbar_init(&x.teacher_full[tid - 16], 1);
+      tc::mbar_init(&x.teacher_free[tid - 16], 1);
+      tc::mbar_init(&x.row_done[tid - 16], kRoleWarps + 1);
+    }
     if (tid >= 32) {
       tc::mbar_init(&x.queue_full[tid - 32], 1);
-      tc::mbar_init(&x.queue_empty[tid - 32], (kGrad ? 2 : 1) * kRoleWarps + kControlWarps);
+      tc::mbar_init(&x.queue_empty[tid - 32], (kGrad ? 2 : 1) * (kRoleWarps + kDistill) + kControlWarps + kDistill);
     }
-    if (tid == 16) tc::mbar_init(&x.response_full, 1);
-    if (tid == 17 || tid == 18) {
-      tc::mbar_init(&x.ticket_full[tid - 17], 1);
-      tc::mbar_init(&x.ticket_free[tid - 17], uint32_t(parts));
+    if (tid == 24) tc::mbar_init(&x.response_full, 1);
+    if (tid == 25 || tid == 26) {
+      tc::mbar_init(&x.ticket_full[tid - 25], 1);
+      tc::mbar_init(&x.ticket_free[tid - 25], uint32_t(parts));
     }
     tc::fence_mbar_init();
   }
+  await_previous();
   __syncthreads();
   if (parts > 1) {  // the barriers of every CTA of the cluster are set before one of them is arrived on
     tc::cluster_arrive();
@@ -761,18 +942,35 @@ __global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRo
   bool ok = true;
   QueueReader reader;
   QueuedRow row;
-  Place buf(parts > 1 ? kBuf / 2 : kBuf), slot(kSlots);
+  Place buf(parts > 1 ? kBuf / 2 : kBuf), slot(kSlots), teach(kTeachers);
+  Place read(buf.size);  // half of the buffers behind buf
+  int ahead = 0;
+  // one of the row's partial results, to every CTA of the cluster (statistics warps and the marker)
+  const auto publish = [&](const Stats& st, int index) {
+    if (kGrad == 0 && ++ahead > buf.size / 2) {
+      ok = ok && warp_wait(&x.coef_full[read.i], read.parity);
+      read.next();
+    }
+    if (ok && lane < parts) {
+      const int to = (buf.i * parts + rank) * kParts + index;
+      if (parts == 1) {
+        x.part[to] = make_float4(st.m, st.s, st.u, 0.f);
+        tc::mbar_arrive(&x.part_full[buf.i]);
+      } else {
+        st_async(&x.part[to], &x.part_full[buf.i], uint32_t(lane), st.m, st.s, st.u);
+      }
+    }
+    buf.next();
+  };
 
-  if (warp < kRoleWarps) {
+  if (warp < kGradWarp) {
     // ------------------------------------------------------------------------------------------- statistics
-    Place read(buf.size);  // half of the buffers behind buf
-    int ahead = 0;
     while ((ok = ok && reader.next(x, row)) && row.row >= 0) {
       if (row.label < 0) continue;
       const RowShare<T> sh(logits + row.row * a.ld, V, per, rank);
       Stats st{-INFINITY, 0.f, 0.f};
       for (int at = 0; at < sh.count && ok; at += kChunk, slot.next()) {
-        ok = warp_wait(&x.full[slot.i], slot.parity);
+        ok = warp_wait(kDistill ? &x.marked[slot.i] : &x.full[slot.i], slot.parity);
         const uint32_t src = ring + uint32_t(slot.i * kChunk + tid) * 16u;
         const int left = sh.count - at - tid;
         uint4 v[kPer];
@@ -793,29 +991,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRo
             if (i * kRoleThreads < left && (j0 < 0 || j0 + E > V)) v[i] = mask_edge<T>(v[i], j0, V);
           }
         }
-        if (kGrad == 0) {  // nobody else reads the chunk
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&x.empty[slot.i]);
-        }
-        add_vectors<T, kPer, true>(st, v, a.k);
+        if (kGrad == 0) free_chunk(&x.empty[slot.i], v, &x.sink[warp]);  // nobody else reads the chunk
+        add_vectors<T, kPer, !kDistill>(st, v, a.k);
       }
-      st = merge_warp<true>(st, a.k);
-      if (kGrad == 0 && ++ahead > buf.size / 2) {
-        ok = ok && warp_wait(&x.coef_full[read.i], read.parity);
-        read.next();
-      }
-      if (ok && lane < parts) {
-        const int to = (buf.i * parts + rank) * kRoleWarps + warp;
-        if (parts == 1) {
-          x.part[to] = make_float4(st.m, st.s, st.u, 0.f);
-          tc::mbar_arrive(&x.part_full[buf.i]);
-        } else {
-          st_async(&x.part[to], &x.part_full[buf.i], uint32_t(lane), st.m, st.s, st.u);
-        }
-      }
-      buf.next();
+      publish(merge_warp<!kDistill>(st, a.k), warp);
     }
-  } else if (warp < 2 * kRoleWarps) {
+  } else if (warp < kControlWarp) {
     // --------------------------------------------------------------------------------------------- gradient
     // (without one its warps leave at once)
     const int tg = tid - kRoleThreads;
@@ -825,13 +1006,14 @@ __global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRo
       const RowShare<T> sh(logits + row.row * a.ld, V, per, rank);
       T* dz = static_cast<T*>(a.dlogits) + row.row * a.ld_d;
       const bool live = row.label >= 0, plain = same && !sh.ragged;
-      RowCoef o{0.f, 0.f, 0.f, 0.f, -1};
+      RowCoef o;
+      o.y = -1;
       if (live) {
         ok = warp_wait(&x.coef_full[buf.i], buf.parity);
         o = x.coef[buf.i];
         buf.next();
       }
-      const int label = o.y < 0 ? -1 : (o.y + sh.off) / E - sh.v0;  // its vector of the share
+      const int label = kDistill || o.y < 0 ? -1 : (o.y + sh.off) / E - sh.v0;  // its vector of the share
       for (int at = 0; at < sh.count && ok; at += kChunk) {
         uint4 v[kPer];
         if (live) {
@@ -839,8 +1021,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRo
           const uint32_t src = ring + uint32_t(slot.i * kChunk + tg) * 16u;
 #pragma unroll
           for (int i = 0; i < kPer; ++i) v[i] = lds16(src + i * kRoleThreads * 16);
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&x.empty[slot.i]);
+          free_chunk(&x.empty[slot.i], v, &x.sink[warp]);
           slot.next();
         }
         const int left = sh.count - at - tg, j0 = (sh.v0 + at + tg) * E - sh.off;
@@ -870,13 +1051,18 @@ __global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRo
         if (label >= at && label < at + kChunk && label < sh.count && (label & (kRoleThreads - 1)) == tg)
           from_f32(dz + o.y, o.at_label);
       }
+      if (kDistill && live) {
+        __syncwarp();
+        if (lane == 0 && ok) tc::mbar_arrive(&x.row_done[teach.i]);
+        teach.next();
+      }
     }
-  } else if (warp < 2 * kRoleWarps + kControlWarps) {
+  } else if (warp < kProducerWarp) {
     // ---------------------------------------------------------------------------------------------- control
     const bool write = rank == 0 && lane == 0;
     // The rows that count are taken in turn (so that one's buffer was last used by a row that this warp, too, has seen
-    // done: a wait by parity cannot tell that use from the one two before), and so are the others.
-    int turn = warp - 2 * kRoleWarps, dead_turn = turn;
+    // done), and so are the others.
+    int turn = warp - kControlWarp, dead_turn = turn;
     while ((ok = ok && reader.next(x, row)) && row.row >= 0) {
       int& next = row.label < 0 ? dead_turn : turn;
       const bool mine = next == 0;
@@ -887,25 +1073,54 @@ __global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRo
         if (write) finish_dead_row(a, t, row.row);
         continue;
       }
-      if (!mine) {
-        buf.next();
-        continue;
-      }
-      // asked for while the row's statistics are still being formed
-      const float zy = to_f32((logits + row.row * a.ld)[row.label]);
-      const PolicyIn in = policy_inputs(t, row.row);
-      ok = wait_cluster(&x.part_full[buf.i], buf.parity);
-      if (!ok) break;
-      if (parts > 1 && lane == 0) tc::mbar_arrive_expect_tx(&x.part_full[buf.i], part_bytes);  // for its next use
-      const Stats st = merge_parts<true>(x.part + buf.i * parts * kRoleWarps, parts * kRoleWarps, a.k);
-      const RowCoef o = finish_row<true, kGrad>(a, t, in, row.row, row.label, zy, st, write);
-      if (lane == 0) {
-        x.coef[buf.i] = o;
-        tc::mbar_arrive(&x.coef_full[buf.i]);
+      if (mine) {
+        RowCoef o;
+        if constexpr (!kDistill) {
+          // asked for while the row's statistics are still being formed
+          const float zy = to_f32((logits + row.row * a.ld)[row.label]);
+          const PolicyIn in = policy_inputs(t, row.row);
+          ok = wait_cluster(&x.part_full[buf.i], buf.parity);
+          if (!ok) break;
+          const Stats st = merge_parts<true>(x.part + buf.i * parts * kParts, parts * kParts, a.k);
+          o = finish_row<true, kGrad>(a, t, in, row.row, row.label, zy, st, write);
+        } else {
+          ok = warp_wait(&x.teacher_full[teach.i], teach.parity);
+          if (!ok) break;
+          const Teacher& te = x.teacher[teach.i];
+          const float mass = x.mass[teach.i], wt = t.weights ? t.weights[row.row] : *t.scale;
+          float zk[kMaxTop / 32];  // the student's logits at the ids
+#pragma unroll
+          for (int i = 0; i < kMaxTop / 32; ++i) {
+            const int k = lane + 32 * i;
+            zk[i] = k < t.K && te.id[k] >= 0 ? to_f32((logits + row.row * a.ld)[te.id[k]]) : 0.f;
+          }
+          ok = wait_cluster(&x.part_full[buf.i], buf.parity);
+          if (!ok) break;
+          const Stats st = merge_parts<false>(x.part + buf.i * parts * kParts, parts * kParts, a.k);
+          float kl = 0.f;
+          const float ls = logf(st.s + st.u);
+#pragma unroll
+          for (int i = 0; i < kMaxTop / 32; ++i) {
+            const int k = lane + 32 * i;
+            if (k >= t.K || te.id[k] < 0) continue;
+            kl = distill_term(kl, te.lp[k], zk[i], st.m, a.temperature, ls);
+          }
+          o = finish_distill_row(a, t, row.row, mass, wt, warp_sum(kl), st, write);
+          if (kGrad == 0) {
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&x.teacher_free[teach.i]);
+          }
+        }
+        if (parts > 1 && lane == 0) tc::mbar_arrive_expect_tx(&x.part_full[buf.i], part_bytes);  // for its next use
+        if (lane == 0) {
+          x.coef[buf.i] = o;
+          tc::mbar_arrive(&x.coef_full[buf.i]);
+        }
       }
       buf.next();
+      teach.next();
     }
-  } else {
+  } else if (warp == kProducerWarp) {
     // --------------------------------------------------------------------------------------------- producer
     Place q(kQueue), tk(2);
     uint32_t response_parity = 0;
@@ -926,14 +1141,18 @@ __global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRo
       const int rows = int(min(int64_t(group_rows), a.n - first));
       int mine = -1;
       if (lane < rows) {
-        const int64_t y = ld_index(a.labels, a.index_dtype, first + lane);
-        mine = y == a.ignore_index ? -1 : (y < 0 || y >= V) ? -2 : int(y);
+        if constexpr (kDistill) {
+          mine = ld_index(t.ids, a.index_dtype, (first + lane) * t.K) < 0 ? -1 : 0;
+        } else {
+          const int64_t y = ld_index(a.labels, a.index_dtype, first + lane);
+          mine = y == a.ignore_index ? -1 : (y < 0 || y >= V) ? -2 : int(y);
+        }
       }
       if (rank == 0) {
         const bool answered = warp_wait(&x.response_full, response_parity);
         response_parity ^= 1u;
         const int64_t cta = answered ? requested_cta(&x.response) : -1;
-        next = cta < 0 ? -1 : int(cta / parts);
+        next = __shfl_sync(0xffffffffu, cta < 0 ? -1 : int(cta / parts), 0);
         ok = ok && answered;
         tc::fence_proxy_async_smem();  // read before the next answer is written there
         __syncwarp();
@@ -960,6 +1179,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRo
         for (int at = 0; at < sh.count && ok; at += kChunk, slot.next()) {
           if (slot.wrapped) ok = warp_wait(&x.empty[slot.i], slot.parity ^ 1u);
           if (lane != 0 || !ok) continue;
+          if (kDistill) tc::fence_proxy_async_smem();  // the marker has written to the slot: the copy comes after
           const uint32_t dst = ring + uint32_t(slot.i * kChunk) * 16u;
           int lo = at, hi = min(at + kChunk, sh.count);
           if (head && lo == 0) {
@@ -981,8 +1201,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRo
       }
       if (parts > 1) {
         ok = wait_cluster(&x.ticket_full[tk.i], tk.parity) && ok;
-        next = x.ticket[tk.i];
-        __syncwarp();
+        next = __shfl_sync(0xffffffffu, x.ticket[tk.i], 0);
         if (lane == 0) arrive_cluster(&x.ticket_free[tk.i], 0);
         tk.next();
       }
@@ -995,6 +1214,126 @@ __global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRo
       for (int i = 0; i < kSlots; ++i)
         if (slot.wrapped || i < slot.i)
           tc::mbar_wait_bounded(&x.full[i], i < slot.i ? slot.parity : slot.parity ^ 1u, 1u << 16);
+  } else if constexpr (kDistill) {
+    if (warp == kTeacherWarp) {
+      // -------------------------------------------------------------------------------------------- teacher
+      while ((ok = ok && reader.next(x, row)) && row.row >= 0) {
+        if (row.label < 0) continue;
+        int id[kMaxTop / 32];
+        float lp[kMaxTop / 32];
+        const float mass = teacher_probabilities(a, t, row.row, rank == 0, id, lp);
+        if (teach.wrapped) ok = warp_wait(&x.teacher_free[teach.i], teach.parity ^ 1u);
+        if (!ok) break;
+        Teacher& te = x.teacher[teach.i];
+#pragma unroll
+        for (int i = 0; i < kMaxTop / 32; ++i) {
+          te.id[lane + 32 * i] = id[i];
+          te.lp[lane + 32 * i] = lp[i];
+        }
+        if (lane == 0) x.mass[teach.i] = mass;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&x.teacher_full[teach.i]);
+        teach.next();
+      }
+    } else if (warp == kMarkerWarp) {
+      // --------------------------------------------------------------------------------------------- marker
+      while ((ok = ok && reader.next(x, row)) && row.row >= 0) {
+        if (row.label < 0) continue;
+        ok = warp_wait(&x.teacher_full[teach.i], teach.parity);
+        if (!ok) break;
+        int id[kMaxTop / 32];
+#pragma unroll
+        for (int i = 0; i < kMaxTop / 32; ++i) id[i] = x.teacher[teach.i].id[lane + 32 * i];
+        const RowShare<T> sh(logits + row.row * a.ld, V, per, rank);
+        Stats st{-INFINITY, 0.f, 0.f};
+        bool again = false;
+        for (int at = 0; at < sh.count && ok; at += kChunk, slot.next()) {
+          ok = warp_wait(&x.full[slot.i], slot.parity);
+          const int lo = (sh.v0 + at) * E - sh.off, hi = (sh.v0 + min(at + kChunk, sh.count)) * E - sh.off;
+          const uint32_t base = ring + uint32_t(slot.i * kChunk) * 16u;
+          uint32_t place[kMaxTop / 32];  // an entry's element in the chunk; a word of the lane's own where it has none
+          bool here[kMaxTop / 32], any = false;
+#pragma unroll
+          for (int i = 0; i < kMaxTop / 32; ++i) {
+            here[i] = id[i] >= 0 && id[i] >= lo && id[i] < hi;
+            place[i] = here[i] ? base + uint32_t(id[i] - lo) * uint32_t(sizeof(T)) : tc::smem_u32(&x.spare[lane]);
+            any |= here[i];
+          }
+          if (__any_sync(0xffffffffu, any)) {
+            // every entry leaves its number; the one that is found there counts, the others are the same id again
+            uint32_t bits[kMaxTop / 32], found[kMaxTop / 32];
+#pragma unroll
+            for (int i = 0; i < kMaxTop / 32; ++i) bits[i] = get_bits<T>(place[i]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kMaxTop / 32; ++i) put_bits<T>(place[i], uint32_t(lane + 32 * i));
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kMaxTop / 32; ++i) found[i] = get_bits<T>(place[i]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kMaxTop / 32; ++i) put_bits<T>(place[i], Vec<T>::kFill);
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&x.marked[slot.i]);
+            float m = st.m;
+#pragma unroll
+            for (int i = 0; i < kMaxTop / 32; ++i) {
+              const bool own = found[i] == uint32_t(lane + 32 * i);
+              again |= here[i] && !own;
+              here[i] = here[i] && own && bits_to_f32<T>(bits[i]) != -INFINITY;
+              if (here[i]) m = fmaxf(m, bits_to_f32<T>(bits[i]));
+            }
+            rescale<false>(st, m, a.k);
+#pragma unroll
+            for (int i = 0; i < kMaxTop / 32; ++i)
+              if (here[i]) st.u += ex2((bits_to_f32<T>(bits[i]) - m) * a.k);
+          } else if (lane == 0) {
+            tc::mbar_arrive(&x.marked[slot.i]);
+          }
+        }
+        again = __any_sync(0xffffffffu, again);
+        if (lane == 0 && kGrad != 0) {
+          x.twice[teach.i] = again;
+          tc::mbar_arrive(&x.row_done[teach.i]);
+        }
+        publish(merge_warp<false>(st, a.k), kRoleWarps);
+        teach.next();
+      }
+    } else if (kGrad != 0) {
+      // -------------------------------------------------------------------------------------------- patcher
+      while ((ok = ok && reader.next(x, row)) && row.row >= 0) {
+        if (row.label < 0) continue;
+        ok = warp_wait(&x.coef_full[buf.i], buf.parity);
+        if (!ok) break;
+        const RowCoef o = x.coef[buf.i];
+        const T* z = logits + row.row * a.ld;
+        const RowShare<T> sh(z, V, per, rank);
+        const Teacher& te = x.teacher[teach.i];
+        int id[kMaxTop / 32];  // the ids of this share
+        float zk[kMaxTop / 32];
+#pragma unroll
+        for (int i = 0; i < kMaxTop / 32; ++i) {
+          id[i] = o.y >= 0 ? te.id[lane + 32 * i] : -1;
+          const int vi = (id[i] + sh.off) / E - sh.v0;
+          if (vi < 0 || vi >= sh.count) id[i] = -1;
+          zk[i] = id[i] >= 0 ? to_f32(z[id[i]]) : 0.f;  // asked for while the gradient is being written
+        }
+        ok = warp_wait(&x.row_done[teach.i], teach.parity);
+        if (!ok) break;
+        const bool twice = x.twice[teach.i] != 0;
+#pragma unroll
+        for (int i = 0; i < kMaxTop / 32; ++i) {
+          if (id[i] < 0) continue;
+          const float p = twice ? mass_at(te.id, te.lp, t.K, id[i]) : expf(te.lp[lane + 32 * i]);
+          const float q = ex2((zk[i] - o.m) * a.k) / o.sum;
+          from_f32(static_cast<T*>(a.dlogits) + row.row * a.ld_d + id[i], o.c * fmaf(q, o.total, -p));
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&x.teacher_free[teach.i]);
+        buf.next();
+        teach.next();
+      }
+    }
   }
   if (!ok && lane == 0) record_device_error(&g_loss_error, kErrLossWaitTimeout);
   if (parts > 1) {  // no CTA leaves while another may still write to its shared memory
@@ -1010,6 +1349,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) policy_stream_kernel(LossRo
 template <typename T, int NT, bool kTail, bool kGrad>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, DistillTerms t, int parts) {
   extern __shared__ float sm[];
+  await_previous();
   const int K = t.K;
   float* tp = sm;                                // [K] teacher logits, then probabilities
   int* id = reinterpret_cast<int*>(sm + K);      // [K] ids, -1 where there is none
@@ -1186,6 +1526,7 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
 __global__ void __launch_bounds__(1024) live_scale_kernel(const void* __restrict__ labels, int index_dtype, int64_t n,
                                                           int64_t stride, bool by_sign, int64_t ignore_index,
                                                           float* __restrict__ scale) {
+  await_previous();
   __shared__ double red[32];
   int64_t c = 0;
   for (int64_t r = threadIdx.x; r < n; r += 1024) {
@@ -1197,8 +1538,9 @@ __global__ void __launch_bounds__(1024) live_scale_kernel(const void* __restrict
 }
 
 // loss = factor * sum_r part[r], in a fixed order (one CTA)
-__global__ void __launch_bounds__(1024) loss_sum_kernel(const float* __restrict__ part, int64_t n, double factor,
+__global__ void __launch_bounds__(1024) loss_sum_kernel(const float* part, int64_t n, double factor,
                                                         float* __restrict__ loss) {
+  await_previous();
   __shared__ double red[32];
   double v = 0.0;
   for (int64_t r = threadIdx.x; r < n; r += 1024) v += double(part[r]);
@@ -1209,6 +1551,7 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* __restrict_
 // One CTA per pair (sequences 2p chosen, 2p + 1 rejected): the log ratios of both, the pair's loss, and
 // d loss / d logp of their tokens.
 __global__ void __launch_bounds__(kSmall) pair_kernel(PairTerms t) {
+  await_previous();
   __shared__ double red[kSmall / 32];
   const int64_t p = blockIdx.x;
   int64_t lo[2], hi[2];
@@ -1291,22 +1634,36 @@ Split choose_scan_split(const LossRows& a) {
   return Split{vecs <= 1024 ? 32 : vecs <= 8192 ? 128 : 256, 1};
 }
 
+// One launch.  `after`: the previous one on the stream is of the same call, and this one's start may overlap its end.
 template <typename... KArgs, typename... Args>
-cudaError_t launch_rows(void (*kernel)(KArgs...), int64_t rows, Split s, bool cluster, size_t smem,
-                        cudaStream_t stream, Args... args) {
+cudaError_t launch(void (*kernel)(KArgs...), int64_t grid, int threads, int cluster, size_t smem, bool after,
+                   cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg = {};
-  if (s.threads == 32) rows = (rows + 3) / 4, s.threads = 128;
-  cfg.gridDim = dim3(unsigned(rows * s.parts));
-  cfg.blockDim = dim3(unsigned(s.threads));
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(unsigned(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = unsigned(s.parts);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = cluster && s.parts > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, args..., s.parts);
+  cudaLaunchAttribute attrs[2] = {};
+  cfg.attrs = attrs;
+  if (after) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attrs[cfg.numAttrs].val.clusterDim.x = unsigned(cluster);
+    attrs[cfg.numAttrs].val.clusterDim.y = attrs[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// ... of a kernel with `parts` CTAs a row as its last argument
+template <typename K, typename... Args>
+cudaError_t launch_rows(K kernel, int64_t rows, Split s, bool cluster, size_t smem, bool after, cudaStream_t stream,
+                        Args... args) {
+  if (s.threads == 32) rows = (rows + 3) / 4, s.threads = 128;
+  return launch(kernel, rows * s.parts, s.threads, cluster ? s.parts : 1, smem, after, stream, args..., s.parts);
 }
 
 // f(T of the logits, threads) as types
@@ -1344,31 +1701,32 @@ Stream choose_stream(const LossRows& a) {
   return {0, 0};
 }
 
-// Rows of one request: as many as make 128 KiB, as long as that leaves every SM eight requests to even out what ignored
-// rows save.
+// Rows of one request: as many as make 128 KiB, as long as that leaves every SM sixteen requests to even out what
+// ignored rows save.
 int64_t group_rows(const LossRows& a, Stream s) {
-  const int64_t chunks = (s.per + kChunk - 1) / kChunk, most = a.n * s.parts / (8 * current_sm_count());
+  const int64_t chunks = (s.per + kChunk - 1) / kChunk, most = a.n * s.parts / (16 * current_sm_count());
   return std::max<int64_t>(1, std::min<int64_t>(8 / chunks, most));
 }
 
-template <typename K>
-cudaError_t launch_stream(K kernel, const LossRows& a, const PolicyTerms& t, Stream s, cudaStream_t stream) {
+template <typename Terms, typename K>
+cudaError_t launch_stream(K kernel, const LossRows& a, const Terms& t, Stream s, bool after, cudaStream_t stream) {
+  using S = Streaming<Terms>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRingBytes));
       e != cudaSuccess)
     return e;
   const int64_t group = group_rows(a, s);
-  return launch_rows(kernel, (a.n + group - 1) / group, Split{kStreamThreads, s.parts}, true, kRingBytes, stream, a, t,
-                     int(group), s.per);
+  return launch_rows(kernel, (a.n + group - 1) / group, Split{S::kThreads, s.parts}, true, kRingBytes, after,
+                     stream, a, t, int(group), s.per);
 }
 
-cudaError_t launch_logp(const LossRows& a, const PolicyTerms& t, cudaStream_t stream) {
+cudaError_t launch_logp(const LossRows& a, const PolicyTerms& t, bool after, cudaStream_t stream) {
   const Stream st = t.row_loss ? choose_stream(a) : Stream{0, 0};
   if (st.parts > 0) {
     const auto go = [&](auto z) {
       using T = decltype(z);
-      if (!a.dlogits) return launch_stream(policy_stream_kernel<T, 0>, a, t, st, stream);
-      return t.entropy_coef != 0.f ? launch_stream(policy_stream_kernel<T, 2>, a, t, st, stream)
-                                   : launch_stream(policy_stream_kernel<T, 1>, a, t, st, stream);
+      if (!a.dlogits) return launch_stream(loss_stream_kernel<T, PolicyTerms, 0>, a, t, st, after, stream);
+      return t.entropy_coef != 0.f ? launch_stream(loss_stream_kernel<T, PolicyTerms, 2>, a, t, st, after, stream)
+                                   : launch_stream(loss_stream_kernel<T, PolicyTerms, 1>, a, t, st, after, stream);
     };
     return a.dtype == KDN_DTYPE_BF16 ? go(__nv_bfloat16{}) : go(float{});
   }
@@ -1376,39 +1734,61 @@ cudaError_t launch_logp(const LossRows& a, const PolicyTerms& t, cudaStream_t st
   return dispatch(a, s, [&](auto z, auto nt) {
     using T = decltype(z);
     constexpr int NT = decltype(nt)::value;
-    const auto go = [&](auto kernel) { return launch_rows(kernel, a.n, s, true, 0, stream, a, t); };
+    const auto go = [&](auto kernel) { return launch_rows(kernel, a.n, s, true, 0, after, stream, a, t); };
     if (!t.row_loss) return go(logp_kernel<T, NT, false, 0>);
     if (!a.dlogits) return go(logp_kernel<T, NT, true, 0>);
     return t.entropy_coef != 0.f ? go(logp_kernel<T, NT, true, 2>) : go(logp_kernel<T, NT, true, 1>);
   });
 }
 
+cudaError_t launch_distill(const LossRows& a, const DistillTerms& t, bool after, cudaStream_t stream) {
+  const Stream st = t.K <= kMaxTop ? choose_stream(a) : Stream{0, 0};
+  if (st.parts > 0) {
+    const auto go = [&](auto z) {
+      using T = decltype(z);
+      return a.dlogits ? launch_stream(loss_stream_kernel<T, DistillTerms, 1>, a, t, st, after, stream)
+                       : launch_stream(loss_stream_kernel<T, DistillTerms, 0>, a, t, st, after, stream);
+    };
+    return a.dtype == KDN_DTYPE_BF16 ? go(__nv_bfloat16{}) : go(float{});
+  }
+  Split s = choose_split(a);
+  s.threads = std::max(s.threads, 128);
+  return dispatch(a, s, [&](auto z, auto nt) {
+    using T = decltype(z);
+    constexpr int NT = decltype(nt)::value < 128 ? 128 : decltype(nt)::value;
+    const auto go = [&](auto kernel) { return launch_rows(kernel, a.n, s, true, size_t(t.K) * 8, after, stream, a, t); };
+    if (t.lse) return a.dlogits ? go(distill_kernel<T, NT, true, true>) : go(distill_kernel<T, NT, true, false>);
+    return a.dlogits ? go(distill_kernel<T, NT, false, true>) : go(distill_kernel<T, NT, false, false>);
+  });
+}
+
 }  // namespace
 
 cudaError_t launch_token_logprobs(const LossRows& a, cudaStream_t stream) {
-  return launch_logp(a, PolicyTerms{}, stream);
+  return launch_logp(a, PolicyTerms{}, false, stream);
 }
 
-cudaError_t launch_token_logprobs_backward(const LossRows& a, const float* dlogps, cudaStream_t stream) {
+cudaError_t launch_token_logprobs_backward(const LossRows& a, const float* dlogps, bool after, cudaStream_t stream) {
   // Nothing ties a row's CTAs together: at most two rounds of 256 threads each.  B200, bf16, 8192 x 32000: 165 us with
   // 256 threads and one CTA a row, 180 with two CTAs, 173 with four of 128 threads, 190 with 512 threads and 4 vectors.
   const int64_t vecs = row_vectors(a);
   Split s{vecs <= 512 ? 32 : vecs <= 128 * kNV ? 128 : 256, 1};
   while (vecs > 4096 * int64_t(s.parts)) s.parts *= 2;
   return dispatch(a, s, [&](auto z, auto nt) {
-    return launch_rows(logp_backward_kernel<decltype(z), decltype(nt)::value>, a.n, s, false, 0, stream, a, dlogps);
+    return launch_rows(logp_backward_kernel<decltype(z), decltype(nt)::value>, a.n, s, false, 0, after, stream, a,
+                       dlogps);
   });
 }
 
 cudaError_t launch_policy_loss(const LossRows& a, const PolicyTerms& t, float* loss, cudaStream_t stream) {
-  if (!t.weights) {
-    live_scale_kernel<<<1, 1024, 0, stream>>>(a.labels, a.index_dtype, a.n, 1, false, a.ignore_index,
-                                              const_cast<float*>(t.scale));
-    if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+  const bool mean = !t.weights;
+  if (mean) {
+    const cudaError_t e = launch(live_scale_kernel, 1, 1024, 1, 0, false, stream, a.labels, a.index_dtype, a.n, 1, false,
+                                 a.ignore_index, const_cast<float*>(t.scale));
+    if (e != cudaSuccess) return e;
   }
-  if (cudaError_t e = launch_logp(a, t, stream); e != cudaSuccess) return e;
-  loss_sum_kernel<<<1, 1024, 0, stream>>>(t.row_loss, a.n, 1.0, loss);
-  return cudaGetLastError();
+  if (cudaError_t e = launch_logp(a, t, mean, stream); e != cudaSuccess) return e;
+  return launch(loss_sum_kernel, 1, 1024, 1, 0, true, stream, t.row_loss, a.n, 1.0, loss);
 }
 
 cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, float* loss, cudaStream_t stream) {
@@ -1416,32 +1796,24 @@ cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, float*
     LossRows f = a;  // forward: log-probabilities and statistics only
     f.dlogits = nullptr;
     f.coef_zero = t.coef;
-    if (cudaError_t e = launch_logp(f, PolicyTerms{}, stream); e != cudaSuccess) return e;
+    if (cudaError_t e = launch_logp(f, PolicyTerms{}, false, stream); e != cudaSuccess) return e;
   }
-  pair_kernel<<<unsigned(t.pairs), kSmall, 0, stream>>>(t);
-  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
-  loss_sum_kernel<<<1, 1024, 0, stream>>>(t.pair_loss, t.pairs, 1.0 / double(t.pairs), loss);
-  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
-  return a.dlogits && a.n > 0 ? launch_token_logprobs_backward(a, t.coef, stream) : cudaSuccess;
+  if (cudaError_t e = launch(pair_kernel, t.pairs, kSmall, 1, 0, a.n > 0, stream, t); e != cudaSuccess) return e;
+  const cudaError_t e = launch(loss_sum_kernel, 1, 1024, 1, 0, true, stream, t.pair_loss, t.pairs,
+                               1.0 / double(t.pairs), loss);
+  if (e != cudaSuccess || !a.dlogits || a.n == 0) return e;
+  return launch_token_logprobs_backward(a, t.coef, true, stream);
 }
 
 cudaError_t launch_distillation_loss(const LossRows& a, const DistillTerms& t, float* loss, cudaStream_t stream) {
-  if (!t.weights) {
-    live_scale_kernel<<<1, 1024, 0, stream>>>(t.ids, a.index_dtype, a.n, t.K, true, 0, const_cast<float*>(t.scale));
-    if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+  const bool mean = !t.weights;
+  if (mean) {
+    const cudaError_t e = launch(live_scale_kernel, 1, 1024, 1, 0, false, stream, t.ids, a.index_dtype, a.n, t.K, true,
+                                 0, const_cast<float*>(t.scale));
+    if (e != cudaSuccess) return e;
   }
-  Split s = choose_split(a);
-  s.threads = std::max(s.threads, 128);
-  const cudaError_t e = dispatch(a, s, [&](auto z, auto nt) {
-    using T = decltype(z);
-    constexpr int NT = decltype(nt)::value < 128 ? 128 : decltype(nt)::value;
-    const auto go = [&](auto kernel) { return launch_rows(kernel, a.n, s, true, size_t(t.K) * 8, stream, a, t); };
-    if (t.lse) return a.dlogits ? go(distill_kernel<T, NT, true, true>) : go(distill_kernel<T, NT, true, false>);
-    return a.dlogits ? go(distill_kernel<T, NT, false, true>) : go(distill_kernel<T, NT, false, false>);
-  });
-  if (e != cudaSuccess) return e;
-  loss_sum_kernel<<<1, 1024, 0, stream>>>(t.row_loss, a.n, 1.0, loss);
-  return cudaGetLastError();
+  if (cudaError_t e = launch_distill(a, t, mean, stream); e != cudaSuccess) return e;
+  return launch(loss_sum_kernel, 1, 1024, 1, 0, true, stream, t.row_loss, a.n, 1.0, loss);
 }
 
 cudaError_t launch_scale_rows(void* x, int dtype, int64_t ld, int64_t n, int64_t V, const float* scale,

@@ -193,6 +193,13 @@ SIZES = [(1, 1), (3, 2), (5, 7), (17, 31), (33, 200), (4, 1000), (9, 4099), (300
          (3, 131072), (1, 262145), (2, 300007)]
 
 
+# rows enough, and long enough, for the kernel that streams them (two rows an SM, more than 32 KiB each), on one CTA a
+# row and on a cluster; every layout of the others
+STREAM = [(300, 16411, torch.bfloat16, "packed"), (300, 8200, torch.float32, "offset"),
+          (311, 40001, torch.bfloat16, "strided"), (300, 40000, torch.float32, "padded"),
+          (297, 80003, torch.bfloat16, "offset"), (297, 80003, torch.float32, "packed")]
+
+
 # ----------------------------------------------------------------------------------------------- log-probabilities
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -338,6 +345,12 @@ def _cuda(*arrays):
 
 
 @gpu
+@pytest.mark.parametrize("n,V,dtype,layout", STREAM)
+def test_policy_loss_streamed(n, V, dtype, layout):
+    test_policy_loss(n, V, layout, dtype)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("layout", LAYOUTS)
 @pytest.mark.parametrize("n,V", SIZES)
@@ -476,6 +489,65 @@ def _teacher(n, V, K, rng, T, dtype=np.float32):
     m = (t / T).max(-1)
     lse = m + np.log(np.exp(t / T - m[:, None]).sum(-1)) - np.log(0.6 + 0.35 * rng.random(n))
     return ids, t, lse.astype(np.float32)
+
+
+@gpu
+@pytest.mark.parametrize("n,V,dtype,layout,K", [(*c, k) for c, k in zip(STREAM, (1, 128, 33, 64, 100, 7))])
+def test_distillation_loss_streamed(n, V, dtype, layout, K):
+    test_distillation_loss(n, V, K, layout, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_streamed_rows_with_infinities_and_repeated_ids(dtype):
+    """The masks of the other tests in rows that are streamed: -inf, nothing left, NaN, ignored rows that hold NaN, the
+    type's lowest value, ids given twice, a masked id."""
+    import kdn_b200 as kdn
+
+    n, V, K, inf = 300, 20000, 40, float("inf")
+    rng = np.random.default_rng(12)
+    z = _logits(n, V, dtype, "packed", seed=21).clone()
+    z[0, 1::2], z[1], z[2, 77], z[3] = -inf, -inf, float("nan"), float("nan")
+    z[4] = torch.finfo(dtype).min
+    z[5, 1:] = -inf
+    y, yd = _labels(n, V, rng, ignored=0)
+    y[:6] = [0, 0, 5, -100, 9, 0]
+    yd = torch.from_numpy(y).cuda()
+    old, adv = -9 - rng.random(n).astype(np.float32), rng.standard_normal(n).astype(np.float32)
+    w = (rng.random(n) / n).astype(np.float32)
+    want = oracle.policy_loss(_np(z), y, old, adv, None, w, 0.2, 0.2, 0.0, 0.01)
+    o, a, wd = _cuda(old, adv, w)
+    loss, logps, H, d = kdn.policy_loss_and_grad(z, yd, o, a, weights=wd, entropy_coef=0.01)
+    fine = [i for i in range(n) if i not in (1, 2)]
+    eps = 2.0 ** -23 * 60 + 2.0 ** -17
+    assert np.isnan(_np(logps)[[1, 2]]).all() and np.isnan(_np(d)[[1, 2]]).all() and torch.isnan(loss)
+    assert np.abs(_np(logps) - want[1])[fine].max() <= eps
+    assert np.abs(_np(H) - want[2])[fine].max() <= eps * (2 + np.log(V))
+    ratio = np.exp(np.clip(want[1] - old, -30, 3))
+    coef = w * (np.abs(adv) * (1 + ratio) + 0.01 * (2 + np.log(V))) + 1e-30
+    _assert_grad(d[fine], want[3][fine], coef[fine], eps, dtype)
+    assert not d[3].any()
+    for tail in (False, True):
+        ids, t, lse = _teacher(n, V, K, rng, 1.0)
+        ids[6, 5] = ids[6, 9] = ids[6, 1]
+        ids[7, :] = V + 1
+        ids[3, 0] = -1
+        z[8, ids[8, 2]] = -inf
+        lse = (np.log(np.exp(t.astype(np.float64)).sum(-1)) + 0.3).astype(np.float32)
+        want = oracle.distillation_loss(_np(z), t, ids, lse if tail else None, w)
+        td, idd, ld = _cuda(t, ids, lse if tail else None)
+        loss, kl, d = kdn.distillation_loss_and_grad(z, td, idd, teacher_lse=ld, weights=wd)
+        got = _np(kl)
+        assert np.isnan(got[[1, 2]]).all() and got[3] == 0 and got[7] == 0 and got[8] == inf
+        rows = [i for i in range(n) if i not in (0, 1, 2, 5, 8)]
+        assert np.abs(got - want[1])[rows].max() <= 30 * (eps + 2.0 ** -23 * 40)
+        assert not d[3].any() and not d[7].any()
+        _assert_grad(d[rows], want[2][rows], 21 * w[rows], eps + 2.0 ** -23 * 40, dtype)
+    import ctypes
+
+    from kdn_b200 import _lib
+    code = ctypes.c_int(0)
+    assert _lib.load().kdn_device_error(_lib.stream_handle(z.device), ctypes.byref(code)) == 0 and code.value == 1
 
 
 @gpu
