@@ -350,7 +350,7 @@ int kdn_varlen_causal_attention(const void* q, const void* k_cache, const void* 
  * Losses over vocabulary logits (no reference entry points; the reference trains with torch's losses, and upcycles a
  * teacher's layers in pipeline/transmute.py).  logits [n, V] (dtype KDN_DTYPE_F32 or KDN_DTYPE_BF16), rows ld elements
  * apart (ld >= V, any ld and any element-aligned start; rows of one 16-byte phase move by vectors).  x = logits /
- * temperature, log q = x - log sum e^x; sums and statistics are fp32.  dlogits (same dtype, rows ld_d apart; must not
+ * temperature (in [1e-6, 1e6]), log q = x - log sum e^x; sums and statistics are fp32.  dlogits (same dtype, rows ld_d apart; must not
  * overlap logits) is the gradient of the loss, rounded once; NULL: no gradient is formed.  logits equal to -inf have
  * probability zero; a row of nothing else, or with a NaN or +inf, gives NaN.
  *
@@ -381,27 +381,27 @@ int kdn_varlen_causal_attention(const void* q, const void* k_cache, const void* 
  * Workspaces: the *_workspace_size entries, 256-byte aligned.
  */
 int kdn_token_logprobs(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
-                       int64_t ignore_index, float* logps, float* row_stats, int64_t n, int64_t V, float temperature,
+                       int64_t ignore_index, float* logps, float* row_stats, int64_t n, int64_t V, double temperature,
                        void* stream);
 int kdn_token_logprobs_backward(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
                                 int64_t ignore_index, const float* row_stats, const float* dlogps, void* dlogits,
-                                int64_t ld_d, int64_t n, int64_t V, float temperature, void* stream);
+                                int64_t ld_d, int64_t n, int64_t V, double temperature, void* stream);
 size_t kdn_policy_loss_workspace_size(int64_t n);
 int kdn_policy_loss(const void* logits, int dtype, int64_t ld, const void* actions, int index_dtype,
                     int64_t ignore_index, const float* old_logps, const float* advantages, const float* ref_logps,
                     const float* weights, float clip_low, float clip_high, float kl_coef, float entropy_coef,
-                    float temperature, float* loss, float* logps, float* entropy, void* dlogits, int64_t ld_d,
+                    double temperature, float* loss, float* logps, float* entropy, void* dlogits, int64_t ld_d,
                     int64_t n, int64_t V, void* workspace, size_t workspace_bytes, void* stream);
 size_t kdn_preference_loss_workspace_size(int64_t n, int64_t pairs);
 int kdn_preference_loss(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
                         int64_t ignore_index, const int64_t* cu_seqlens, int64_t pairs, const float* ref_logps,
-                        float beta, float label_smoothing, int length_normalised, float temperature, float* loss,
+                        float beta, float label_smoothing, int length_normalised, double temperature, float* loss,
                         float* log_ratios, float* logps, void* dlogits, int64_t ld_d, int64_t n, int64_t V,
                         void* workspace, size_t workspace_bytes, void* stream);
 size_t kdn_distillation_loss_workspace_size(int64_t n);
 int kdn_distillation_loss(const void* logits, int dtype, int64_t ld, const void* teacher_logits, int teacher_dtype,
                           const void* teacher_ids, int index_dtype, int32_t top, const float* teacher_lse,
-                          const float* weights, float temperature, float* loss, float* divergence, void* dlogits,
+                          const float* weights, double temperature, float* loss, float* divergence, void* dlogits,
                           int64_t ld_d, int64_t n, int64_t V, void* workspace, size_t workspace_bytes, void* stream);
 int kdn_scale_rows(void* x, int dtype, int64_t ld, int64_t n, int64_t V, const float* scale, void* stream);
 

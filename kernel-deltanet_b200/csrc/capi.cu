@@ -3,6 +3,7 @@
 // Every entry point validates its arguments, enqueues work on the caller's
 // stream and returns a status code; failures leave a message in a thread-local
 // buffer read by kdn_last_error().  Nothing here allocates device memory.
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -124,13 +125,13 @@ int check_affine_dims(int64_t batch, int32_t D, int32_t dv, bool need_dv) {
 
 // arguments that every loss over logits shares
 int check_loss_rows(const void* logits, int dtype, int64_t ld, const void* dlogits, int64_t ld_d, int64_t n, int64_t V,
-                    int index_dtype, float temperature) {
+                    int index_dtype, double temperature) {
   if (!valid_dtype(dtype)) return fail(KDN_ERR_INVALID, "bad dtype");
   if (index_dtype != KDN_INDEX_I32 && index_dtype != KDN_INDEX_I64) return fail(KDN_ERR_INVALID, "bad index dtype");
   if (n < 0 || n >= (int64_t(1) << 28)) return fail(KDN_ERR_INVALID, "n=%lld outside [0, 2^28)", (long long)n);
   if (V < 1 || V > (int64_t(1) << 30)) return fail(KDN_ERR_INVALID, "V=%lld outside [1, 2^30]", (long long)V);
-  if (!(temperature > 0.f) || temperature > 3e38f)
-    return fail(KDN_ERR_INVALID, "temperature must be positive and finite");
+  if (!(temperature >= 1e-6 && temperature <= 1e6))
+    return fail(KDN_ERR_INVALID, "temperature=%g outside [1e-6, 1e6]", temperature);
   if (n == 0) return KDN_OK;
   if (!logits) return fail(KDN_ERR_INVALID, "logits is NULL");
   if (ld < V) return fail(KDN_ERR_INVALID, "ld=%lld below V=%lld", (long long)ld, (long long)V);
@@ -145,8 +146,15 @@ int check_loss_rows(const void* logits, int dtype, int64_t ld, const void* dlogi
   return KDN_OK;
 }
 
+// x > 0 as its nearest float, and as the sum of two of which the second is positive
+void split_float(double x, float* nearest, float* hi, float* lo) {
+  *nearest = float(x);
+  *hi = double(*nearest) < x ? *nearest : nextafterf(*nearest, 0.f);
+  *lo = float(x - double(*hi));
+}
+
 kdn::LossRows loss_rows(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
-                        int64_t ignore_index, void* dlogits, int64_t ld_d, int64_t n, int64_t V, float temperature) {
+                        int64_t ignore_index, void* dlogits, int64_t ld_d, int64_t n, int64_t V, double temperature) {
   kdn::LossRows a{};
   a.logits = logits;
   a.dtype = dtype;
@@ -157,8 +165,8 @@ kdn::LossRows loss_rows(const void* logits, int dtype, int64_t ld, const void* l
   a.n = n;
   a.V = V;
   a.temperature = temperature;
-  a.k = float(1.4426950408889634 / double(temperature));
-  a.inv_t = float(1.0 / double(temperature));
+  split_float(1.4426950408889634 / temperature, &a.k, &a.k_hi, &a.k_lo);
+  split_float(1.0 / temperature, &a.inv_t, &a.inv_hi, &a.inv_lo);
   a.dlogits = dlogits;
   a.ld_d = ld_d;
   return a;
@@ -872,7 +880,7 @@ int kdn_fork_state(void* states, int64_t num_slots, int64_t bytes_per_slot, int6
 }
 
 int kdn_token_logprobs(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
-                       int64_t ignore_index, float* logps, float* row_stats, int64_t n, int64_t V, float temperature,
+                       int64_t ignore_index, float* logps, float* row_stats, int64_t n, int64_t V, double temperature,
                        void* stream) {
   if (int rc = check_loss_rows(logits, dtype, ld, nullptr, 0, n, V, index_dtype, temperature)) return rc;
   if (n == 0) return ok();
@@ -887,7 +895,7 @@ int kdn_token_logprobs(const void* logits, int dtype, int64_t ld, const void* la
 
 int kdn_token_logprobs_backward(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
                                 int64_t ignore_index, const float* row_stats, const float* dlogps, void* dlogits,
-                                int64_t ld_d, int64_t n, int64_t V, float temperature, void* stream) {
+                                int64_t ld_d, int64_t n, int64_t V, double temperature, void* stream) {
   if (int rc = check_loss_rows(logits, dtype, ld, dlogits, ld_d, n, V, index_dtype, temperature)) return rc;
   if (n == 0) return ok();
   if (!labels || !row_stats || !dlogps || !dlogits)
@@ -904,7 +912,7 @@ size_t kdn_policy_loss_workspace_size(int64_t n) { return n < 0 ? 0 : 256 + alig
 int kdn_policy_loss(const void* logits, int dtype, int64_t ld, const void* actions, int index_dtype,
                     int64_t ignore_index, const float* old_logps, const float* advantages, const float* ref_logps,
                     const float* weights, float clip_low, float clip_high, float kl_coef, float entropy_coef,
-                    float temperature, float* loss, float* logps, float* entropy, void* dlogits, int64_t ld_d,
+                    double temperature, float* loss, float* logps, float* entropy, void* dlogits, int64_t ld_d,
                     int64_t n, int64_t V, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_loss_rows(logits, dtype, ld, dlogits, ld_d, n, V, index_dtype, temperature)) return rc;
   if (!(clip_low >= 0.f && clip_low <= 1.f) || !(clip_high >= 0.f))
@@ -942,13 +950,13 @@ int kdn_policy_loss(const void* logits, int dtype, int64_t ld, const void* actio
 
 size_t kdn_preference_loss_workspace_size(int64_t n, int64_t pairs) {
   if (n < 0 || pairs < 1) return 0;
-  return align256(2 * sizeof(float) * size_t(n)) + align256(sizeof(float) * size_t(n)) +
+  return 256 + align256(2 * sizeof(float) * size_t(n)) + align256(sizeof(float) * size_t(n)) +
          align256(sizeof(float) * size_t(pairs));
 }
 
 int kdn_preference_loss(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,
                         int64_t ignore_index, const int64_t* cu_seqlens, int64_t pairs, const float* ref_logps,
-                        float beta, float label_smoothing, int length_normalised, float temperature, float* loss,
+                        float beta, float label_smoothing, int length_normalised, double temperature, float* loss,
                         float* log_ratios, float* logps, void* dlogits, int64_t ld_d, int64_t n, int64_t V,
                         void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_loss_rows(logits, dtype, ld, dlogits, ld_d, n, V, index_dtype, temperature)) return rc;
@@ -960,26 +968,23 @@ int kdn_preference_loss(const void* logits, int dtype, int64_t ld, const void* l
   if (n > 0 && (!labels || !logps)) return fail(KDN_ERR_INVALID, "labels/logps is NULL");
   if (int rc = check_loss_workspace(workspace, workspace_bytes, kdn_preference_loss_workspace_size(n, pairs))) return rc;
   kdn::LossRows a = loss_rows(logits, dtype, ld, labels, index_dtype, ignore_index, dlogits, ld_d, n, V, temperature);
-  char* ws = static_cast<char*>(workspace);
+  char* ws = static_cast<char*>(workspace) + 256;
   a.logps = logps;
   a.stats = reinterpret_cast<float*>(ws);
   ws += align256(2 * sizeof(float) * size_t(n));
   kdn::PairTerms t{};
   t.coef = reinterpret_cast<float*>(ws);
   t.pair_loss = reinterpret_cast<float*>(ws + align256(sizeof(float) * size_t(n)));
+  t.pairs_done = static_cast<unsigned*>(workspace);
+  t.loss = loss;
   t.cu = cu_seqlens;
   t.pairs = pairs;
-  t.n = n;
-  t.labels = labels;
-  t.index_dtype = index_dtype;
-  t.ignore_index = ignore_index;
-  t.logps = logps;
   t.ref = ref_logps;
   t.beta = beta;
   t.smoothing = label_smoothing;
   t.normalise = length_normalised != 0;
   t.log_ratios = log_ratios;
-  cudaError_t e = kdn::launch_preference_loss(a, t, loss, static_cast<cudaStream_t>(stream));
+  cudaError_t e = kdn::launch_preference_loss(a, t, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "preference loss launch");
   return ok();
 }
@@ -988,7 +993,7 @@ size_t kdn_distillation_loss_workspace_size(int64_t n) { return kdn_policy_loss_
 
 int kdn_distillation_loss(const void* logits, int dtype, int64_t ld, const void* teacher_logits, int teacher_dtype,
                           const void* teacher_ids, int index_dtype, int32_t top, const float* teacher_lse,
-                          const float* weights, float temperature, float* loss, float* divergence, void* dlogits,
+                          const float* weights, double temperature, float* loss, float* divergence, void* dlogits,
                           int64_t ld_d, int64_t n, int64_t V, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_loss_rows(logits, dtype, ld, dlogits, ld_d, n, V, index_dtype, temperature)) return rc;
   if (!valid_dtype(teacher_dtype)) return fail(KDN_ERR_INVALID, "bad dtype");
@@ -1013,7 +1018,7 @@ int kdn_distillation_loss(const void* logits, int dtype, int64_t ld, const void*
   t.lse = teacher_lse;
   t.weights = weights;
   t.scale = static_cast<float*>(workspace);
-  t.t2 = temperature * temperature;
+  t.t2 = float(temperature * temperature);
   t.row_loss = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
   t.divergence = divergence;
   cudaError_t e = kdn::launch_distillation_loss(a, t, loss, st);
@@ -1022,7 +1027,7 @@ int kdn_distillation_loss(const void* logits, int dtype, int64_t ld, const void*
 }
 
 int kdn_scale_rows(void* x, int dtype, int64_t ld, int64_t n, int64_t V, const float* scale, void* stream) {
-  if (int rc = check_loss_rows(x, dtype, ld, nullptr, 0, n, V, KDN_INDEX_I64, 1.f)) return rc;
+  if (int rc = check_loss_rows(x, dtype, ld, nullptr, 0, n, V, KDN_INDEX_I64, 1.0)) return rc;
   if (n == 0) return ok();
   if (!scale) return fail(KDN_ERR_INVALID, "scale is NULL");
   cudaError_t e = kdn::launch_scale_rows(x, dtype, ld, n, V, scale, static_cast<cudaStream_t>(stream));

@@ -190,20 +190,22 @@ struct LossRows {
   int index_dtype;
   int64_t ignore_index;
   int64_t n, V;
-  float temperature;
-  float k;      // log2(e) / temperature
-  float inv_t;  // 1 / temperature
+  double temperature;
+  // log2(e) / temperature and its reciprocal: rounded, and as the sum of two floats of which the second is positive (so
+  // that -inf times either is -inf)
+  float k, k_hi, k_lo, inv_t, inv_hi, inv_lo;
   float* logps;        // [n]
   float* stats;        // [n, 2]: largest logit, sum of e^((z - largest) / T); may be null
   void* dlogits;       // [n, V], rows ld_d elements apart; null: no gradient
   int64_t ld_d;
   float* coef_zero;    // [n] set to zero by the forward pass; may be null
+  unsigned* pairs_done;  // set to zero with them
 };
 struct PolicyTerms {
   const float* old_logps;   // [n]
   const float* advantages;  // [n]
   const float* ref_logps;   // [n] or null
-  const float* weights;     // [n] or null: *scale
+  const float* weights;     // [n] or null: *scale, or (null) the mean of few rows
   const float* scale;
   float clip_low, clip_high, kl_coef, entropy_coef;
   float* row_loss;  // [n] weight x loss of each row (null: no loss, log-probabilities only)
@@ -211,17 +213,15 @@ struct PolicyTerms {
 };
 struct PairTerms {
   const int64_t* cu;  // [2 pairs + 1]
-  int64_t pairs, n;
-  const void* labels;
-  int index_dtype;
-  int64_t ignore_index;
-  const float* logps;  // [n]
+  int64_t pairs;
   const float* ref;    // [n] or null
   float beta, smoothing;
   bool normalise;
   float* log_ratios;  // [2 pairs]
   float* pair_loss;   // [pairs]
   float* coef;        // [n] d loss / d logp
+  unsigned* pairs_done;  // zero before the first pair
+  float* loss;
 };
 struct DistillTerms {
   const void* logits;  // [n, K] teacher logits (dtype)
@@ -229,7 +229,7 @@ struct DistillTerms {
   const void* ids;     // [n, K] (the rows' index_dtype)
   int K;
   const float* lse;      // [n] or null: the teacher renormalised over its K entries
-  const float* weights;  // [n] or null: *scale
+  const float* weights;  // [n] or null: *scale, or (null) the mean of few rows
   const float* scale;
   float t2;  // T^2
   float* row_loss;        // [n]
@@ -238,9 +238,9 @@ struct DistillTerms {
 cudaError_t launch_token_logprobs(const LossRows& a, cudaStream_t stream);
 // `after`: the previous launch on the stream is of the same call
 cudaError_t launch_token_logprobs_backward(const LossRows& a, const float* dlogps, bool after, cudaStream_t stream);
-cudaError_t launch_policy_loss(const LossRows& a, const PolicyTerms& t, float* loss, cudaStream_t stream);
-cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, float* loss, cudaStream_t stream);
-cudaError_t launch_distillation_loss(const LossRows& a, const DistillTerms& t, float* loss, cudaStream_t stream);
+cudaError_t launch_policy_loss(const LossRows& a, PolicyTerms t, float* loss, cudaStream_t stream);
+cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, cudaStream_t stream);
+cudaError_t launch_distillation_loss(const LossRows& a, DistillTerms t, float* loss, cudaStream_t stream);
 cudaError_t launch_scale_rows(void* x, int dtype, int64_t ld, int64_t n, int64_t V, const float* scale,
                               cudaStream_t stream);
 cudaError_t loss_read_error(cudaStream_t stream, int* code);

@@ -243,7 +243,7 @@ struct Share {
   }
   __device__ __forceinline__ void store(int vi, const float2* g) const {
     if (same && whole(vi)) {
-      *reinterpret_cast<uint4*>(dz + (vi * E - off)) = Vec<T>::pack(g);
+      __stcs(reinterpret_cast<uint4*>(dz + (vi * E - off)), Vec<T>::pack(g));  // not read again here
       return;
     }
 #pragma unroll
@@ -268,6 +268,12 @@ struct Cta {
   }
 };
 
+// x / T + c in fp32, rounded once: the quotient's two halves (see LossRows; not through log2(e) / T or one rounded 1 / T,
+// whose error would show in a log-probability)
+__device__ __forceinline__ float over_t(const LossRows& a, float x, float c) {
+  return fmaf(x, a.inv_hi, fmaf(x, a.inv_lo, c));
+}
+
 // Largest logit m, sum of exponentials below it, and a second sum (see its use) of a part of a row.
 struct Stats {
   float m, s, u;
@@ -275,10 +281,11 @@ struct Stats {
 
 // The statistics of two parts together.  kMoment: u is sum e^d d (base 2), which a change of m shifts; else a sum
 // like s.  A part without a finite logit has m = -inf and sums of zero (or NaN) and is left as it is.
+// (The factor is expf's, which errs to both sides; ex2.approx truncates, and a sum is rescaled several times.)
 template <bool kMoment>
-__device__ __forceinline__ void rescale(Stats& a, float m, float k) {
+__device__ __forceinline__ void rescale(Stats& a, float m, const LossRows& r) {
   if (a.m == m) return;
-  const float d = (a.m - m) * k, f = ex2(d);
+  const float d = (a.m - m) * r.k, f = expf(over_t(r, a.m - m, 0.f));
   if constexpr (kMoment)
     a.u = f == 0.f ? 0.f : f * fmaf(a.s, d, a.u);
   else
@@ -289,11 +296,11 @@ __device__ __forceinline__ void rescale(Stats& a, float m, float k) {
 
 // the statistics of a warp's lanes together
 template <bool kMoment>
-__device__ __forceinline__ Stats merge_warp(Stats a, float k) {
+__device__ __forceinline__ Stats merge_warp(Stats a, const LossRows& r) {
   float m = a.m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  rescale<kMoment>(a, m, k);
+  rescale<kMoment>(a, m, r);
   a.s = warp_sum(a.s);
   a.u = warp_sum(a.u);
   return a;
@@ -301,37 +308,37 @@ __device__ __forceinline__ Stats merge_warp(Stats a, float k) {
 
 // ... of `count` parts in shared memory, by every warp that asks
 template <bool kMoment>
-__device__ __forceinline__ Stats merge_parts(const float4* p, int count, float k) {
+__device__ __forceinline__ Stats merge_parts(const float4* p, int count, const LossRows& r) {
   const int lane = threadIdx.x & 31;
   Stats a{-INFINITY, 0.f, 0.f};
   for (int i = lane; i < count; i += 32) {
     const float4 t = p[i];
     Stats b{t.x, t.y, t.z};
     const float m = fmaxf(a.m, b.m);
-    rescale<kMoment>(a, m, k);
-    rescale<kMoment>(b, m, k);
+    rescale<kMoment>(a, m, r);
+    rescale<kMoment>(b, m, r);
     a.s += b.s;
     a.u += b.u;
   }
-  return merge_warp<kMoment>(a, k);
+  return merge_warp<kMoment>(a, r);
 }
 
 // ... of all threads of the row's cluster
 template <int NT, bool kMoment>
-__device__ __forceinline__ Stats merge_rows(Stats a, float k, int rank, int parts) {
-  a = merge_warp<kMoment>(a, k);
+__device__ __forceinline__ Stats merge_rows(Stats a, const LossRows& r, int rank, int parts) {
+  a = merge_warp<kMoment>(a, r);
   if constexpr (NT == 32) return a;
   __shared__ float4 part[NT / 32];
   __shared__ float4 remote[kMaxCluster];
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float4(a.m, a.s, a.u, 0.f);
   __syncthreads();
-  a = merge_parts<kMoment>(part, NT / 32, k);
+  a = merge_parts<kMoment>(part, NT / 32, r);
   if (parts > 1) {
     if (threadIdx.x < unsigned(parts))
       tc::st_cluster_v4(tc::mapa(tc::smem_u32(&remote[rank]), threadIdx.x), a.m, a.s, a.u, 0.f);
     tc::cluster_arrive();
     tc::cluster_wait();
-    a = merge_parts<kMoment>(remote, parts, k);
+    a = merge_parts<kMoment>(remote, parts, r);
   }
   return a;
 }
@@ -361,7 +368,7 @@ struct PolicyIn {
 };
 __device__ __forceinline__ PolicyIn policy_inputs(const PolicyTerms& t, int64_t r) {
   if (!t.row_loss) return PolicyIn{};
-  return PolicyIn{t.weights ? t.weights[r] : *t.scale, t.advantages[r], t.old_logps[r],
+  return PolicyIn{t.weights ? t.weights[r] : t.scale ? *t.scale : 0.f, t.advantages[r], t.old_logps[r],
                   t.ref_logps ? t.ref_logps[r] : 0.f};
 }
 __device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, const PolicyIn& in, float logp, float H) {
@@ -382,6 +389,23 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, const Poli
   return p;
 }
 
+// 1 / (rows that count) for a few rows, by every warp that asks: rows whose label is not ignore_index, or (ids) whose
+// first id is not negative.
+constexpr int64_t kFewRows = 256;
+__device__ __forceinline__ float mean_of_few(const LossRows& a, const void* ids, int K) {
+  int live = 0;
+  for (int64_t r = threadIdx.x & 31; r < a.n; r += 32)
+    live += ids ? ld_index(ids, a.index_dtype, r * K) >= 0 : ld_index(a.labels, a.index_dtype, r) != a.ignore_index;
+  live = __reduce_add_sync(0xffffffffu, live);
+  return live > 0 ? 1.f / float(live) : 0.f;
+}
+
+// before the pairs are formed: no coefficient yet, no pair done
+__device__ __forceinline__ void zero_coef(const LossRows& a, int64_t r) {
+  a.coef_zero[r] = 0.f;
+  if (r == 0) *a.pairs_done = 0u;
+}
+
 // What the gradient of a row needs: dz_j = 2^d (A + B d) with d = (z_j - m) k, and dz_y; for the distillation loss the
 // entries at the teacher's ids are c (total q - p), q = 2^d / sum.
 struct RowCoef {
@@ -396,14 +420,13 @@ struct RowCoef {
 template <bool kEntropy, int kGrad>
 __device__ __forceinline__ RowCoef finish_row(const LossRows& a, const PolicyTerms& t, const PolicyIn& in, int64_t r,
                                               int y, float zy, const Stats& st, bool write) {
-  // to base e and with a division, not through k = log2(e) / T, whose rounding would show in a log-probability (and
-  // products rounded on their own, so that calls with and without a gradient give the same bits)
+  // products rounded on their own, so that calls with and without a gradient give the same bits
   const float dy = __fmul_rn(zy - st.m, a.k), ls = logf(st.s);
-  const float logp = __fsub_rn(__fdiv_rn(zy - st.m, a.temperature), ls);
+  const float logp = over_t(a, zy - st.m, -ls);
   if (write) {
     a.logps[r] = logp;
     if (a.stats) a.stats[2 * r] = st.m, a.stats[2 * r + 1] = st.s;
-    if (a.coef_zero) a.coef_zero[r] = 0.f;
+    if (a.coef_zero) zero_coef(a, r);
   }
   RowCoef o{st.m, 0.f, 0.f, 0.f, -1, 0.f, 0.f, 0.f};
   if (!t.row_loss) return o;
@@ -426,7 +449,7 @@ __device__ __forceinline__ RowCoef finish_row(const LossRows& a, const PolicyTer
 __device__ __forceinline__ void finish_dead_row(const LossRows& a, const PolicyTerms& t, int64_t r) {
   a.logps[r] = 0.f;
   if (a.stats) a.stats[2 * r] = 0.f, a.stats[2 * r + 1] = 1.f;
-  if (a.coef_zero) a.coef_zero[r] = 0.f;
+  if (a.coef_zero) zero_coef(a, r);
   if (t.entropy) t.entropy[r] = 0.f;
   if (t.row_loss) t.row_loss[r] = 0.f;
 }
@@ -437,9 +460,9 @@ __device__ __forceinline__ void finish_dead_row(const LossRows&, const DistillTe
 }
 
 // p (log p - log q) of one teacher entry, added to kl; an entry of probability zero adds nothing
-__device__ __forceinline__ float distill_term(float kl, float lp, float z, float m, float temperature, float ls) {
+__device__ __forceinline__ float distill_term(const LossRows& a, float kl, float lp, float z, float m, float ls) {
   const float p = expf(lp);
-  return p != 0.f ? fmaf(p, lp - ((z - m) / temperature - ls), kl) : kl;
+  return p != 0.f ? fmaf(p, lp - over_t(a, z - m, -ls), kl) : kl;
 }
 
 // the teacher's probability at an id that is given more than once
@@ -469,7 +492,7 @@ __device__ __forceinline__ RowCoef finish_distill_row(const LossRows& a, const D
   }
   if (mass < 0.f || weight == 0.f) return o;
   o.y = 0;
-  o.c = weight * a.temperature;
+  o.c = weight * float(a.temperature);
   o.total = mass + pr;
   o.A = o.c * (o.total - (pr > 0.f && qr != 0.f ? pr / qr : 0.f)) / o.sum;
   return o;
@@ -511,7 +534,7 @@ __device__ __forceinline__ float teacher_probabilities(const LossRows& a, const 
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if (id[i] < 0) continue;
-    lp[i] = t.lse ? fmaf(lp[i], a.inv_t, -lse) : fmaf(lp[i] - m, a.inv_t, -s);
+    lp[i] = t.lse ? over_t(a, lp[i], -lse) : over_t(a, lp[i] - m, -s);
     mass += expf(lp[i]);
   }
   mass = warp_sum(mass);
@@ -543,15 +566,22 @@ __device__ __forceinline__ void add_at(float2* g, int e, float c) {
   }
 }
 
+// log2(e) / T in two halves: with one, its rounding moves every exponent of a row the same way, and the log of the row's
+// sum by as much as 1e-6.
+struct Log2Scale {
+  float hi, lo;
+};
+
 // The statistics of N vectors: s = sum 2^d and (kMoment) u = sum 2^d d with d = (z - base) k.
 template <typename T, int N, bool kMoment>
-__device__ __forceinline__ void accumulate(const uint4* v, float base, float k, float& s_out, float& u_out) {
+__device__ __forceinline__ void accumulate(const uint4* v, float base, Log2Scale k, float& s_out, float& u_out) {
   float2 s = make_float2(0.f, 0.f), u = make_float2(0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int j = 0; j < Vec<T>::E / 2; ++j) {
-      const float2 d = mul2(Vec<T>::minus(v[i], j, base), make_float2(k, k));
+      const float2 z = Vec<T>::minus(v[i], j, base);
+      const float2 d = fma2(z, make_float2(k.hi, k.hi), mul2(z, make_float2(k.lo, k.lo)));
       const float2 e = make_float2(ex2(d.x), ex2(d.y));
       s = add2(s, e);
       if constexpr (kMoment)  // a logit of -inf adds 0 x -1000, not 0 x -inf
@@ -563,11 +593,11 @@ __device__ __forceinline__ void accumulate(const uint4* v, float base, float k, 
 
 // `st` with N more vectors
 template <typename T, int N, bool kMoment>
-__device__ __forceinline__ void add_vectors(Stats& st, const uint4* v, float k) {
+__device__ __forceinline__ void add_vectors(Stats& st, const uint4* v, const LossRows& a) {
   const float m = fmaxf(st.m, Vec<T>::template largest<N>(v));
-  rescale<kMoment>(st, m, k);
+  rescale<kMoment>(st, m, a);
   float s, u;
-  accumulate<T, N, kMoment>(v, m == -INFINITY ? 0.f : m, k, s, u);  // without a finite logit: 2^-inf each
+  accumulate<T, N, kMoment>(v, m == -INFINITY ? 0.f : m, Log2Scale{a.k_hi, a.k_lo}, s, u);  // without a finite logit: 2^-inf each
   st.s += s;
   st.u += u;
 }
@@ -592,7 +622,7 @@ __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
   }
   if (parts > 1) tc::cluster_arrive();
   const float zy = to_f32(w.z[y]);
-  const PolicyIn in = policy_inputs(t, r);
+  PolicyIn in = policy_inputs(t, r);
   uint4 v[kNV];
   auto load = [&](int at) {
 #pragma unroll
@@ -605,10 +635,11 @@ __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
   Stats st{-INFINITY, 0.f, 0.f};
   for (int q = 0; q < rounds; ++q) {
     load(w.v0 + q * NT * kNV);
-    add_vectors<T, kNV, kEntropy>(st, v, a.k);
+    add_vectors<T, kNV, kEntropy>(st, v, a);
   }
+  if (t.row_loss && !t.weights && !t.scale) in.w = mean_of_few(a, nullptr, 0);
   if (parts > 1) tc::cluster_wait();  // every CTA of the cluster runs: their shared memory may be written
-  st = merge_rows<NT, kEntropy>(st, a.k, rank, parts);
+  st = merge_rows<NT, kEntropy>(st, a, rank, parts);
   const RowCoef o = finish_row<kEntropy, kGrad>(a, t, in, r, int(y), zy, st, first);
   if constexpr (kGrad != 0) {
     if (o.y < 0) {
@@ -636,8 +667,8 @@ template <typename T, int NT>
 __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
     logp_backward_kernel(LossRows a, const float* dlogps, int parts) {
   await_previous();
-  const int64_t r = Cta<NT>::row(parts);
-  if (r >= a.n) return;
+  const int64_t r = a.n - 1 - Cta<NT>::row(parts);  // what the forward pass read last may still be in L2
+  if (r < 0) return;
   const int tid = int(threadIdx.x) % NT;
   const Share<T> w(a, r, int(blockIdx.x % unsigned(parts)), parts);
   const int64_t y = row_label(a, r, tid == 0);
@@ -992,9 +1023,9 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           }
         }
         if (kGrad == 0) free_chunk(&x.empty[slot.i], v, &x.sink[warp]);  // nobody else reads the chunk
-        add_vectors<T, kPer, !kDistill>(st, v, a.k);
+        add_vectors<T, kPer, !kDistill>(st, v, a);
       }
-      publish(merge_warp<!kDistill>(st, a.k), warp);
+      publish(merge_warp<!kDistill>(st, a), warp);
     }
   } else if (warp < kControlWarp) {
     // --------------------------------------------------------------------------------------------- gradient
@@ -1081,7 +1112,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           const PolicyIn in = policy_inputs(t, row.row);
           ok = wait_cluster(&x.part_full[buf.i], buf.parity);
           if (!ok) break;
-          const Stats st = merge_parts<true>(x.part + buf.i * parts * kParts, parts * kParts, a.k);
+          const Stats st = merge_parts<true>(x.part + buf.i * parts * kParts, parts * kParts, a);
           o = finish_row<true, kGrad>(a, t, in, row.row, row.label, zy, st, write);
         } else {
           ok = warp_wait(&x.teacher_full[teach.i], teach.parity);
@@ -1096,14 +1127,14 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           }
           ok = wait_cluster(&x.part_full[buf.i], buf.parity);
           if (!ok) break;
-          const Stats st = merge_parts<false>(x.part + buf.i * parts * kParts, parts * kParts, a.k);
+          const Stats st = merge_parts<false>(x.part + buf.i * parts * kParts, parts * kParts, a);
           float kl = 0.f;
           const float ls = logf(st.s + st.u);
 #pragma unroll
           for (int i = 0; i < kMaxTop / 32; ++i) {
             const int k = lane + 32 * i;
             if (k >= t.K || te.id[k] < 0) continue;
-            kl = distill_term(kl, te.lp[k], zk[i], st.m, a.temperature, ls);
+            kl = distill_term(a, kl, te.lp[k], zk[i], st.m, ls);
           }
           o = finish_distill_row(a, t, row.row, mass, wt, warp_sum(kl), st, write);
           if (kGrad == 0) {
@@ -1283,7 +1314,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
               here[i] = here[i] && own && bits_to_f32<T>(bits[i]) != -INFINITY;
               if (here[i]) m = fmaxf(m, bits_to_f32<T>(bits[i]));
             }
-            rescale<false>(st, m, a.k);
+            rescale<false>(st, m, a);
 #pragma unroll
             for (int i = 0; i < kMaxTop / 32; ++i)
               if (here[i]) st.u += ex2((bits_to_f32<T>(bits[i]) - m) * a.k);
@@ -1296,7 +1327,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           x.twice[teach.i] = again;
           tc::mbar_arrive(&x.row_done[teach.i]);
         }
-        publish(merge_warp<false>(st, a.k), kRoleWarps);
+        publish(merge_warp<false>(st, a), kRoleWarps);
         teach.next();
       }
     } else if (kGrad != 0) {
@@ -1398,7 +1429,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
       sum = logf(warp_sum(sum));
     }
     for (int k = lane; k < K; k += 32) {
-      const float lp = t.lse ? fmaf(tp[k], a.inv_t, -t.lse[r]) : fmaf(tp[k] - tm, a.inv_t, -sum);
+      const float lp = t.lse ? over_t(a, tp[k], -t.lse[r]) : over_t(a, tp[k] - tm, -sum);
       tp[k] = id[k] < 0 ? -INFINITY : lp;
       if (id[k] >= 0) ps += expf(lp);
     }
@@ -1425,13 +1456,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
         twice = 1;
       } else if (kTail) {
         const float zk = to_f32(w.z[id[k]]), m = fmaxf(st.m, zk);
-        rescale<false>(st, m, a.k);
+        rescale<false>(st, m, a);
         st.u += zk == -INFINITY ? 0.f : ex2((zk - m) * a.k);
       }
     }
     __syncthreads();
     const float m = fmaxf(st.m, Vec<T>::template largest<kNV>(v));
-    rescale<false>(st, m, a.k);
+    rescale<false>(st, m, a);
     const float b = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < kNV; ++i) {
@@ -1448,23 +1479,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
           continue;
         }
       }
-      accumulate<T, 1, false>(v + i, b, a.k, s, u);
+      accumulate<T, 1, false>(v + i, b, Log2Scale{a.k_hi, a.k_lo}, s, u);
       st.s += s;
     }
   }
   if (parts > 1) tc::cluster_wait();
-  st = merge_rows<NT, false>(st, a.k, rank, parts);
+  st = merge_rows<NT, false>(st, a, rank, parts);
   const float S = kTail ? st.s + st.u : st.s, ls = logf(S), ps = ts[0];
   // what is left of both; where the student has nothing left, a rest of the size of the sum's rounding is none
   const float qr = kTail ? st.s / S : 1.f;
   float pr = kTail ? fmaxf(1.f - ps, 0.f) : 0.f;
   if (qr == 0.f && pr < 0x1p-20f) pr = 0.f;
-  const float wt = t.weights ? t.weights[r] : *t.scale;
+  const float wt = t.weights ? t.weights[r] : t.scale ? *t.scale : mean_of_few(a, t.ids, K);
   if (rank == 0 && tid < 32) {
     float kl = 0.f;
     for (int k = lane; k < K; k += 32) {
-      const float lp = tp[k], p = expf(lp);
-      if (p != 0.f) kl = fmaf(p, lp - ((to_f32(w.z[id[k]]) - st.m) / a.temperature - ls), kl);
+      if (id[k] >= 0) kl = distill_term(a, kl, tp[k], to_f32(w.z[id[k]]), st.m, ls);
     }
     kl = warp_sum(kl);
     if (pr > 0.f) kl += pr * (logf(pr) - logf(qr));
@@ -1478,7 +1508,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
       w.template zero<NT>(tid);
       return;
     }
-    const float c = wt * a.temperature, A = ps + pr, R = pr > 0.f && qr != 0.f ? pr / qr : 0.f;
+    const float c = wt * float(a.temperature), A = ps + pr, R = pr > 0.f && qr != 0.f ? pr / qr : 0.f;
     const float f = c * (A - R) / S;
     for (int q = rounds - 1; q >= 0; --q) {
       if (q < rounds - 1) load(w.v0 + q * NT * kNV);
@@ -1549,8 +1579,8 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* part, int64
 }
 
 // One CTA per pair (sequences 2p chosen, 2p + 1 rejected): the log ratios of both, the pair's loss, and
-// d loss / d logp of their tokens.
-__global__ void __launch_bounds__(kSmall) pair_kernel(PairTerms t) {
+// d loss / d logp of their tokens.  The CTA that is done last adds the pairs' losses, in the pairs' order.
+__global__ void __launch_bounds__(kSmall) pair_kernel(LossRows a, PairTerms t) {
   await_previous();
   __shared__ double red[kSmall / 32];
   const int64_t p = blockIdx.x;
@@ -1559,15 +1589,20 @@ __global__ void __launch_bounds__(kSmall) pair_kernel(PairTerms t) {
   for (int i = 0; i < 2; ++i) {
     lo[i] = t.cu[2 * p + i];
     hi[i] = t.cu[2 * p + i + 1];
-    if (lo[i] < 0 || hi[i] > t.n || hi[i] < lo[i]) {  // offsets out of range: the sequence counts as empty
+    if (lo[i] < 0 || hi[i] > a.n || hi[i] < lo[i]) {  // offsets out of range: the sequence counts as empty
       if (threadIdx.x == 0) record_device_error(&g_loss_error, kErrSlotOutOfRange);
       lo[i] = hi[i] = 0;
     }
     double v = 0.0, c = 0.0;
     for (int64_t r = lo[i] + threadIdx.x; r < hi[i]; r += kSmall) {
-      if (ld_index(t.labels, t.index_dtype, r) == t.ignore_index) continue;
-      v += double(t.logps[r]) - (t.ref ? double(t.ref[r]) : 0.0);
+      const int64_t y = ld_index(a.labels, a.index_dtype, r);
+      if (y == a.ignore_index) continue;
       c += 1.0;
+      if (y < 0 || y >= a.V) continue;  // recorded by the forward kernel
+      // from the row's statistics, and not from its log-probability in fp32: a log ratio is a sum of differences of near
+      // values
+      const double z = double(ld_as_f32(a.logits, a.dtype, r * a.ld + y)), m = double(a.stats[2 * r]);
+      v += (z - m) / a.temperature - log(double(a.stats[2 * r + 1])) - (t.ref ? double(t.ref[r]) : 0.0);
     }
     sum[i] = block_sum_f64(v, red);
     cnt[i] = t.normalise ? fmax(block_sum_f64(c, red), 1.0) : 1.0;
@@ -1587,6 +1622,18 @@ __global__ void __launch_bounds__(kSmall) pair_kernel(PairTerms t) {
     const float c = float((i == 0 ? dh : -dh) * double(t.beta) / (double(t.pairs) * cnt[i]));
     for (int64_t r = lo[i] + threadIdx.x; r < hi[i]; r += kSmall) t.coef[r] = c;
   }
+  __shared__ bool last;
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(t.pairs_done, 1u) == unsigned(t.pairs - 1);
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last) return;
+  double v = 0.0;
+  for (int64_t q = threadIdx.x; q < t.pairs; q += kSmall) v += double(__ldcg(t.pair_loss + q));
+  v = block_sum_f64(v, red);
+  if (threadIdx.x == 0) *t.loss = float(v / double(t.pairs));
 }
 
 // x *= *scale, row by row; nothing is read or written where the scale is one
@@ -1780,8 +1827,9 @@ cudaError_t launch_token_logprobs_backward(const LossRows& a, const float* dlogp
   });
 }
 
-cudaError_t launch_policy_loss(const LossRows& a, const PolicyTerms& t, float* loss, cudaStream_t stream) {
-  const bool mean = !t.weights;
+cudaError_t launch_policy_loss(const LossRows& a, PolicyTerms t, float* loss, cudaStream_t stream) {
+  if (t.weights || a.n <= kFewRows) t.scale = nullptr;  // few rows: their own kernel counts
+  const bool mean = t.scale != nullptr;
   if (mean) {
     const cudaError_t e = launch(live_scale_kernel, 1, 1024, 1, 0, false, stream, a.labels, a.index_dtype, a.n, 1, false,
                                  a.ignore_index, const_cast<float*>(t.scale));
@@ -1791,22 +1839,22 @@ cudaError_t launch_policy_loss(const LossRows& a, const PolicyTerms& t, float* l
   return launch(loss_sum_kernel, 1, 1024, 1, 0, true, stream, t.row_loss, a.n, 1.0, loss);
 }
 
-cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, float* loss, cudaStream_t stream) {
-  if (a.n > 0) {
-    LossRows f = a;  // forward: log-probabilities and statistics only
-    f.dlogits = nullptr;
-    f.coef_zero = t.coef;
-    if (cudaError_t e = launch_logp(f, PolicyTerms{}, false, stream); e != cudaSuccess) return e;
-  }
-  if (cudaError_t e = launch(pair_kernel, t.pairs, kSmall, 1, 0, a.n > 0, stream, t); e != cudaSuccess) return e;
-  const cudaError_t e = launch(loss_sum_kernel, 1, 1024, 1, 0, true, stream, t.pair_loss, t.pairs,
-                               1.0 / double(t.pairs), loss);
+cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, cudaStream_t stream) {
+  LossRows f = a;  // forward: log-probabilities and statistics only
+  f.dlogits = nullptr;
+  f.coef_zero = t.coef;
+  f.pairs_done = t.pairs_done;
+  cudaError_t e = a.n > 0 ? launch_logp(f, PolicyTerms{}, false, stream)
+                          : cudaMemsetAsync(t.pairs_done, 0, sizeof(unsigned), stream);
+  if (e != cudaSuccess) return e;
+  e = launch(pair_kernel, t.pairs, kSmall, 1, 0, a.n > 0, stream, a, t);
   if (e != cudaSuccess || !a.dlogits || a.n == 0) return e;
   return launch_token_logprobs_backward(a, t.coef, true, stream);
 }
 
-cudaError_t launch_distillation_loss(const LossRows& a, const DistillTerms& t, float* loss, cudaStream_t stream) {
-  const bool mean = !t.weights;
+cudaError_t launch_distillation_loss(const LossRows& a, DistillTerms t, float* loss, cudaStream_t stream) {
+  if (t.weights || a.n <= kFewRows) t.scale = nullptr;  // few rows: their own kernel counts
+  const bool mean = t.scale != nullptr;
   if (mean) {
     const cudaError_t e = launch(live_scale_kernel, 1, 1024, 1, 0, false, stream, t.ids, a.index_dtype, a.n, t.K, true,
                                  0, const_cast<float*>(t.scale));

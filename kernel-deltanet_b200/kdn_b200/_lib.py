@@ -48,6 +48,7 @@ _I32 = ctypes.c_int32
 _INT = ctypes.c_int
 _U32 = ctypes.c_uint32
 _F32 = ctypes.c_float
+_F64 = ctypes.c_double
 
 # name -> (restype, argtypes); the list is also what the export test checks
 SIGNATURES = {
@@ -86,16 +87,16 @@ SIGNATURES = {
     "kdn_add_rmsnorm": (_INT, [_P, _P, _INT, _P, _INT, _P, _P, _I64, _I32, ctypes.c_float, _P]),
     "kdn_swiglu": (_INT, [_P, _P, _INT, _I64, _I32, _P]),
     "kdn_mixer_inputs": (_INT, [_P, _INT, _I64, _I32, _I32, _I64, _P, _INT, _P, _I64, _P, _P, _P, _P, _P, _P]),
-    "kdn_token_logprobs": (_INT, [_P, _INT, _I64, _P, _INT, _I64, _P, _P, _I64, _I64, _F32, _P]),
-    "kdn_token_logprobs_backward": (_INT, [_P, _INT, _I64, _P, _INT, _I64, _P, _P, _P, _I64, _I64, _I64, _F32, _P]),
+    "kdn_token_logprobs": (_INT, [_P, _INT, _I64, _P, _INT, _I64, _P, _P, _I64, _I64, _F64, _P]),
+    "kdn_token_logprobs_backward": (_INT, [_P, _INT, _I64, _P, _INT, _I64, _P, _P, _P, _I64, _I64, _I64, _F64, _P]),
     "kdn_policy_loss_workspace_size": (ctypes.c_size_t, [_I64]),
-    "kdn_policy_loss": (_INT, [_P, _INT, _I64, _P, _INT, _I64, _P, _P, _P, _P, _F32, _F32, _F32, _F32, _F32, _P, _P, _P,
+    "kdn_policy_loss": (_INT, [_P, _INT, _I64, _P, _INT, _I64, _P, _P, _P, _P, _F32, _F32, _F32, _F32, _F64, _P, _P, _P,
                                _P, _I64, _I64, _I64, _P, ctypes.c_size_t, _P]),
     "kdn_preference_loss_workspace_size": (ctypes.c_size_t, [_I64, _I64]),
-    "kdn_preference_loss": (_INT, [_P, _INT, _I64, _P, _INT, _I64, _P, _I64, _P, _F32, _F32, _INT, _F32, _P, _P, _P, _P,
+    "kdn_preference_loss": (_INT, [_P, _INT, _I64, _P, _INT, _I64, _P, _I64, _P, _F32, _F32, _INT, _F64, _P, _P, _P, _P,
                                    _I64, _I64, _I64, _P, ctypes.c_size_t, _P]),
     "kdn_distillation_loss_workspace_size": (ctypes.c_size_t, [_I64]),
-    "kdn_distillation_loss": (_INT, [_P, _INT, _I64, _P, _INT, _P, _INT, _I32, _P, _P, _F32, _P, _P, _P, _I64, _I64,
+    "kdn_distillation_loss": (_INT, [_P, _INT, _I64, _P, _INT, _P, _INT, _I32, _P, _P, _F64, _P, _P, _P, _I64, _I64,
                                      _I64, _P, ctypes.c_size_t, _P]),
     "kdn_scale_rows": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _P]),
     "kdn_copy_rows": (_INT, [_P, ctypes.c_size_t, _P, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t, _P]),

@@ -31,15 +31,22 @@ from torch.autograd.function import once_differentiable
 from .. import _lib
 
 _INDEX = {torch.int64: _lib.KDN_INDEX_I64, torch.int32: _lib.KDN_INDEX_I32}
+_DTYPE = {torch.float32: _lib.KDN_DTYPE_F32, torch.bfloat16: _lib.KDN_DTYPE_BF16}
+_entries: dict = {}
 
 
 def _call(name: str, dev: torch.device, *args) -> None:
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    """The C entry on dev's current stream.  A call of a few rows takes longer on the host than on the GPU: the entry is
+    looked up once, and the stream's handle is asked for directly."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
+    i = dev.index
+    if torch._C._cuda_getDevice() == i:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     if rc:
         _lib.check(rc, name)
 
@@ -48,7 +55,7 @@ def _rows(logits: torch.Tensor) -> torch.Tensor:
     """[..., V] -> [n, V] with unit-stride rows (a view wherever the strides allow one)."""
     if not logits.is_cuda:
         raise RuntimeError("kdn_b200 runs on CUDA tensors only (no CPU fallback)")
-    if logits.dtype not in (torch.float32, torch.bfloat16):
+    if logits.dtype not in _DTYPE:
         raise RuntimeError(f"logits must be float32 or bfloat16, got {logits.dtype}")
     if logits.dim() < 2 or logits.shape[-1] < 1:
         raise RuntimeError(f"logits must be [..., vocab], got {tuple(logits.shape)}")
@@ -105,8 +112,10 @@ def _f32(shape, dev: torch.device) -> torch.Tensor:
     return torch.empty(shape, device=dev, dtype=torch.float32)
 
 
-def _workspace(size: int, dev: torch.device) -> torch.Tensor:
-    return torch.empty(size, device=dev, dtype=torch.uint8)
+def _beside(workspace: int, dev: torch.device, *sizes: int):
+    """A workspace of `workspace` bytes (a multiple of 256) and float32 outputs of the given sizes, in one allocation."""
+    w = workspace >> 2
+    return torch.empty(w + sum(sizes), device=dev, dtype=torch.float32).split_with_sizes((w, *sizes))
 
 
 def _scalar_grad(holder: list, dloss: torch.Tensor) -> torch.Tensor:
@@ -117,7 +126,7 @@ def _scalar_grad(holder: list, dloss: torch.Tensor) -> torch.Tensor:
     g = holder.pop()
     if g.numel():
         scale = dloss.to(torch.float32)
-        _call("kdn_scale_rows", g.device, g.data_ptr(), _lib.dtype_code(g), _ld(g), g.shape[0], g.shape[1],
+        _call("kdn_scale_rows", g.device, g.data_ptr(), _DTYPE[g.dtype], _ld(g), g.shape[0], g.shape[1],
               scale.data_ptr())
     return g
 
@@ -131,7 +140,7 @@ def _token_logprobs(z, y, temperature, ignore_index, keep_stats):
     n, V = z.shape
     logps = _f32(n, z.device)
     stats = _f32((n, 2), z.device) if keep_stats else None
-    _call("kdn_token_logprobs", z.device, z.data_ptr(), _lib.dtype_code(z), _ld(z), y.data_ptr(), _INDEX[y.dtype],
+    _call("kdn_token_logprobs", z.device, z.data_ptr(), _DTYPE[z.dtype], _ld(z), y.data_ptr(), _INDEX[y.dtype],
           ignore_index, logps.data_ptr(), _lib.ptr(stats), n, V, temperature)
     return logps, stats
 
@@ -176,7 +185,7 @@ def token_logprobs_backward(logits: torch.Tensor, labels: torch.Tensor, row_stat
     d = _per_row(dlogps, (n,), z.device, "dlogps")
     st = _per_row(row_stats, (n, 2), z.device, "row_stats")
     g = _grad_rows(z)
-    _call("kdn_token_logprobs_backward", z.device, z.data_ptr(), _lib.dtype_code(z), _ld(z), y.data_ptr(),
+    _call("kdn_token_logprobs_backward", z.device, z.data_ptr(), _DTYPE[z.dtype], _ld(z), y.data_ptr(),
           _INDEX[y.dtype], int(ignore_index), st.data_ptr(), d.data_ptr(), g.data_ptr(), _ld(g), n, V,
           float(temperature))
     return g
@@ -186,11 +195,11 @@ def token_logprobs_backward(logits: torch.Tensor, labels: torch.Tensor, row_stat
 def _policy(z, y, old, adv, ref, w, clip_low, clip_high, kl_coef, entropy_coef, temperature, ignore_index, with_grad):
     n, V = z.shape
     dev = z.device
-    loss, logps, entropy = _f32((), dev), _f32(n, dev), _f32(n, dev)
-    g = _grad_rows(z) if with_grad else None
     size = 256 + (4 * n + 255) // 256 * 256  # kdn_policy_loss_workspace_size
-    ws = _workspace(size, dev)
-    _call("kdn_policy_loss", dev, z.data_ptr(), _lib.dtype_code(z), _ld(z), y.data_ptr(), _INDEX[y.dtype], ignore_index,
+    ws, logps, entropy = _beside(size, dev, n, n)
+    loss = _f32((), dev)
+    g = _grad_rows(z) if with_grad else None
+    _call("kdn_policy_loss", dev, z.data_ptr(), _DTYPE[z.dtype], _ld(z), y.data_ptr(), _INDEX[y.dtype], ignore_index,
           old.data_ptr(), adv.data_ptr(), _lib.ptr(ref), _lib.ptr(w), clip_low, clip_high, kl_coef, entropy_coef,
           temperature, loss.data_ptr(), logps.data_ptr(), entropy.data_ptr(), _lib.ptr(g),
           _ld(g) if with_grad else 0, n, V, ws.data_ptr(), size)
@@ -241,6 +250,8 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logps: torch.Te
         loss, logps, entropy = _PolicyLoss.apply(*args)
     else:
         loss, logps, entropy, _ = _policy(*args, False)
+    if logits.dim() == 2:
+        return loss, logps, entropy
     shape = logits.shape[:-1]
     return loss, logps.view(shape), entropy.view(shape)
 
@@ -266,11 +277,11 @@ def _preference(z, y, cu, ref, beta, label_smoothing, length_normalised, tempera
     n, V = z.shape
     dev = z.device
     pairs = (cu.numel() - 1) // 2
-    loss, log_ratios, logps = _f32((), dev), _f32(2 * pairs, dev), _f32(n, dev)
+    size = 256 + sum((b + 255) // 256 * 256 for b in (8 * n, 4 * n, 4 * pairs))  # kdn_preference_loss_workspace_size
+    ws, log_ratios, logps = _beside(size, dev, 2 * pairs, n)
+    loss = _f32((), dev)
     g = _grad_rows(z) if with_grad else None
-    size = int(_lib.load().kdn_preference_loss_workspace_size(n, pairs))
-    ws = _workspace(size, dev)
-    _call("kdn_preference_loss", dev, z.data_ptr(), _lib.dtype_code(z), _ld(z), y.data_ptr(), _INDEX[y.dtype],
+    _call("kdn_preference_loss", dev, z.data_ptr(), _DTYPE[z.dtype], _ld(z), y.data_ptr(), _INDEX[y.dtype],
           ignore_index, cu.data_ptr(), pairs, _lib.ptr(ref), beta, label_smoothing, length_normalised, temperature,
           loss.data_ptr(), log_ratios.data_ptr(), logps.data_ptr(), _lib.ptr(g), _ld(g) if with_grad else 0, n, V,
           ws.data_ptr(), size)
@@ -336,11 +347,11 @@ def preference_loss_and_grad(logits: torch.Tensor, labels: torch.Tensor, cu_seql
 def _distillation(z, t, ids, lse, w, temperature, with_grad):
     n, V = z.shape
     dev = z.device
-    loss, divergence = _f32((), dev), _f32(n, dev)
-    g = _grad_rows(z) if with_grad else None
     size = 256 + (4 * n + 255) // 256 * 256  # kdn_distillation_loss_workspace_size
-    ws = _workspace(size, dev)
-    _call("kdn_distillation_loss", dev, z.data_ptr(), _lib.dtype_code(z), _ld(z), t.data_ptr(), _lib.dtype_code(t),
+    ws, divergence = _beside(size, dev, n)
+    loss = _f32((), dev)
+    g = _grad_rows(z) if with_grad else None
+    _call("kdn_distillation_loss", dev, z.data_ptr(), _DTYPE[z.dtype], _ld(z), t.data_ptr(), _DTYPE[t.dtype],
           ids.data_ptr(), _INDEX[ids.dtype], t.shape[-1], _lib.ptr(lse), _lib.ptr(w), temperature, loss.data_ptr(),
           divergence.data_ptr(), _lib.ptr(g), _ld(g) if with_grad else 0, n, V, ws.data_ptr(), size)
     return loss, divergence, g

@@ -93,6 +93,8 @@ def test_loss_argument_checks(lib):
     assert po(old=None) == 1 and po(adv=None) == 1 and po(loss=None) == 1
     assert po(wsb=16) == 4 and po(ws=None) == 4 and po(ws=264) == 1
     assert lib.kdn_policy_loss_workspace_size(4) == 512 and lib.kdn_policy_loss_workspace_size(-1) == 0
+    assert lib.kdn_distillation_loss_workspace_size(65) == 768
+    assert lib.kdn_preference_loss_workspace_size(33, 65) == 256 + 512 + 256 + 512
     pr = lambda **kw: lib.kdn_preference_loss(*[kw.get(k, d) for k, d in (
         ("z", P), ("dt", 1), ("ld", 100), ("y", P), ("it", 1), ("ig", -100), ("cu", P), ("pairs", 2), ("ref", None),
         ("beta", 0.1), ("eps", 0.0), ("norm", 0), ("T", 1.0), ("loss", P), ("lr", P), ("lp", P), ("g", Q),
