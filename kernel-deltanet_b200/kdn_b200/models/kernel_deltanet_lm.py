@@ -16,6 +16,9 @@ Here the same model runs as a serving engine over packed, ragged batches:
 * ``decode_step(tokens, cache)`` -- one token per sequence -> logits [num_seqs, vocab]: the
   libkdn decode step (read-out before the update, state updated in place) per Kernel-DeltaNet
   layer, cached attention per anchor layer.
+* ``hidden_states(input_ids, cu_seqlens)`` and ``score(input_ids, cu_seqlens)`` -- every position of a packed batch: the
+  LM head's inputs, and the log-probability of each next token (libkdn token_logprobs), as the preference and policy
+  losses take them of a reference or a sampling model.
 * ``generate`` (same arguments as the reference; temperature 0 is greedy), ``forward``
   (uniform [B, T] batch -> all logits, + cross-entropy with targets) and
   ``prefill_and_init_states`` keep the reference surface.
@@ -34,6 +37,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..kernels.losses import token_logprobs
 from ..layers.hybrid_kernel_deltanet_block import HybridKernelDeltaNetBlock, Linear, RMSNorm
 
 
@@ -190,6 +194,33 @@ class KernelDeltaNetLM(nn.Module):
         """A CUDA graph of one decode step on `cache` (see DecodeGraph)."""
         return DecodeGraph(self, cache, greedy)
 
+    # ------------------------------------------------------------------ scoring
+    @torch.no_grad()
+    def hidden_states(self, input_ids: torch.Tensor, cu_seqlens: Union[torch.Tensor, Sequence[int]]) -> torch.Tensor:
+        """Packed sequences [total_tokens] with offsets cu_seqlens [B + 1] -> what the LM head reads at every position
+        [total_tokens, d_model]: the blocks' output after the final norm."""
+        cu = [int(c) for c in (cu_seqlens.tolist() if torch.is_tensor(cu_seqlens) else cu_seqlens)]
+        B = len(cu) - 1
+        lens = [cu[i + 1] - cu[i] for i in range(B)]
+        if B < 1 or cu[0] != 0 or min(lens) < 1 or cu[-1] != input_ids.numel():
+            raise ValueError("cu_seqlens must run from 0 to the number of tokens in steps of at least one")
+        dev = self.embed.weight.device
+        cu_dev = torch.tensor(cu, device=dev, dtype=torch.int64)
+        x, delta = self._prefill_body(self.embed(input_ids.to(dev).reshape(-1)), cu, cu_dev, self.new_cache(B, max(lens)),
+                                      torch.arange(B, device=dev), torch.ones(B, dtype=torch.bool))
+        return self.final_norm(x) if delta is None else self.final_norm.add_forward(x, delta)[1]
+
+    @torch.no_grad()
+    def score(self, input_ids: torch.Tensor, cu_seqlens: Union[torch.Tensor, Sequence[int]], temperature: float = 1.0,
+              chunk_tokens: int = 8192) -> torch.Tensor:
+        """Log-probability of every next token: entry t is log p(input_ids[t + 1] | its sequence up to t), and 0 at the
+        last token of a sequence [total_tokens] float32 -- the layout of logits' rows, which predict the token after
+        them.  Logits exist for `chunk_tokens` rows at a time."""
+        h = self.hidden_states(input_ids, cu_seqlens)
+        labels = next_token_labels(input_ids.to(h.device), cu_seqlens)
+        return torch.cat([token_logprobs(self.lm_head(h[i:i + chunk_tokens]), labels[i:i + chunk_tokens], temperature)
+                          for i in range(0, h.shape[0], chunk_tokens)])
+
     # ------------------------------------------------------------------ reference surface
     def forward(self, input_ids: torch.Tensor, targets: Optional[torch.Tensor] = None
                 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
@@ -253,6 +284,16 @@ class KernelDeltaNetLM(nn.Module):
         if ragged:
             return [torch.cat([p.to(gen.device), g]) for p, g in zip(prompts, gen.unbind(0))]
         return torch.cat([prompt_ids.to(gen.device), gen], dim=1)
+
+
+def next_token_labels(input_ids: torch.Tensor, cu_seqlens: Union[torch.Tensor, Sequence[int]],
+                      ignore_index: int = -100) -> torch.Tensor:
+    """The label of every row of a packed batch's logits: the token after it, ignore_index at a sequence's last token."""
+    ids = input_ids.reshape(-1)
+    labels = torch.roll(ids, -1)
+    ends = torch.as_tensor(cu_seqlens, device=ids.device)[1:].to(torch.int64) - 1
+    labels[ends] = ignore_index
+    return labels
 
 
 class DecodeGraph:
