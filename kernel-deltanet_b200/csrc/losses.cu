@@ -294,15 +294,22 @@ __device__ __forceinline__ void rescale(Stats& a, float m, const LossRows& r) {
   a.m = m;
 }
 
-// the statistics of a warp's lanes together
-template <bool kMoment>
+// the largest of a warp's values (none is NaN), in the order of their bits as integers
+__device__ __forceinline__ float warp_max(float x) {
+  const int i = __float_as_int(x);
+  const int m = __reduce_max_sync(0xffffffffu, i ^ ((i >> 31) & 0x7fffffff));
+  return __int_as_float(m ^ ((m >> 31) & 0x7fffffff));
+}
+
+// the statistics of a warp's lanes together; kLeft > 1: of lanes of equal index modulo kLeft, about the warp's maximum
+template <bool kMoment, int kLeft = 1>
 __device__ __forceinline__ Stats merge_warp(Stats a, const LossRows& r) {
-  float m = a.m;
+  rescale<kMoment>(a, warp_max(a.m), r);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  rescale<kMoment>(a, m, r);
-  a.s = warp_sum(a.s);
-  a.u = warp_sum(a.u);
+  for (int o = 16; o >= kLeft; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+  }
   return a;
 }
 
@@ -525,8 +532,7 @@ __device__ __forceinline__ float teacher_probabilities(const LossRows& a, const 
     m = fmaxf(m, lp[i]);
   }
   const float lse = t.lse ? t.lse[r] : 0.f;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  m = warp_max(m);
 #pragma unroll
   for (int i = 0; i < N; ++i)
     if (id[i] >= 0) s += ex2((lp[i] - m) * a.k);
@@ -719,7 +725,7 @@ __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
 // cannot tell a use from the one two before.  Every wait is bounded; after one that gave up a role ends,
 // kErrLossWaitTimeout is recorded, and the CTA returns when its copies have landed.
 constexpr int kPer = 4;                // vectors that a thread of a role takes at a time
-constexpr int kBuf = 16;               // rows between a partial result and its use (8 in a cluster), see Exchange
+constexpr int kBuf = 8;                // rows between a partial result and its use, see Exchange
 constexpr int kQueue = 32;             // rows between the producer and the last of the other roles
 constexpr int kRoleThreads = 256;      // of the statistics and of the gradient role
 constexpr int kRoleWarps = kRoleThreads / 32;
@@ -736,7 +742,8 @@ constexpr size_t kRingBytes = size_t(kSlots) * kChunk * 16;
 template <typename Terms>
 struct Streaming {
   static constexpr bool kDistill = std::is_same_v<Terms, DistillTerms>;
-  static constexpr int kParts = kRoleWarps + (kDistill ? 1 : 0);  // partial results of a row in a CTA
+  static constexpr int kMarkers = kDistill ? 1 : 0;
+  static constexpr int kPartLanes = kDistill ? 1 : 8;  // partial results of a statistics warp (1 in a cluster)
   static constexpr int kThreads = 2 * kRoleThreads + 32 * (kControlWarps + 1 + (kDistill ? 3 : 0));
 };
 
@@ -760,7 +767,8 @@ struct Teacher {
 template <bool kDistill>
 struct Exchange {
   uint4 response;                                                  // of a request for more rows
-  float4 part[kBuf / 2 * kMaxCluster * (kRoleWarps + kDistill)];   // (m, s, u) of each statistics warp of the cluster
+  // (m, s, u) of the statistics warps (of a few lanes of each, or one for each of every CTA of a cluster) and the marker
+  float4 part[kBuf * kMaxCluster * (kRoleWarps + kDistill)];
   QueuedRow queue[kQueue];
   RowCoef coef[kBuf];
   Teacher teacher[kDistill ? kTeachers : 1];
@@ -927,7 +935,8 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
     loss_stream_kernel(LossRows a, Terms t, int group_rows, int per, int parts) {
   extern __shared__ __align__(128) uint8_t ring_mem[];
   constexpr bool kDistill = Streaming<Terms>::kDistill;
-  constexpr int E = Vec<T>::E, kParts = Streaming<Terms>::kParts;
+  constexpr int E = Vec<T>::E, kMarkers = Streaming<Terms>::kMarkers;
+  constexpr int kPartLanes = Streaming<Terms>::kPartLanes;
   // warps: statistics, gradient, control, producer, teacher, marker, patcher
   constexpr int kGradWarp = kRoleWarps, kControlWarp = 2 * kRoleWarps, kProducerWarp = kControlWarp + kControlWarps;
   constexpr int kTeacherWarp = kProducerWarp + 1, kMarkerWarp = kProducerWarp + 2;
@@ -936,7 +945,8 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
   const int rank = int(blockIdx.x % unsigned(parts)), V = int(a.V);
   const uint32_t ring = tc::smem_u32(ring_mem);
   const T* logits = static_cast<const T*>(a.logits);
-  const uint32_t part_bytes = uint32_t(kParts * parts) * 16u;
+  const int row_parts = parts == 1 ? kRoleWarps * kPartLanes + kMarkers : parts * (kRoleWarps + kMarkers);
+  const uint32_t part_bytes = uint32_t(row_parts) * 16u;
   if (tid < 64) {  // a few barriers a thread
     if (tid < kSlots) {
       tc::mbar_init(&x.full[tid], 1);
@@ -944,7 +954,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
       tc::mbar_init(&x.marked[tid], 1);
     }
     if (tid < kBuf) {
-      tc::mbar_init(&x.part_full[tid], parts == 1 ? kParts : 1);
+      tc::mbar_init(&x.part_full[tid], parts == 1 ? kRoleWarps + kMarkers : 1);
       if (parts > 1) tc::mbar_arrive_expect_tx(&x.part_full[tid], part_bytes);
       tc::mbar_init(&x.coef_full[tid], 1);
     }
@@ -973,23 +983,22 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
   bool ok = true;
   QueueReader reader;
   QueuedRow row;
-  Place buf(parts > 1 ? kBuf / 2 : kBuf), slot(kSlots), teach(kTeachers);
+  Place buf(kBuf), slot(kSlots), teach(kTeachers);
   Place read(buf.size);  // half of the buffers behind buf
   int ahead = 0;
-  // one of the row's partial results, to every CTA of the cluster (statistics warps and the marker)
-  const auto publish = [&](const Stats& st, int index) {
+  // a warp's partial results of the row (statistics warps, then the marker): lanes [0, lanes), or to every CTA of the cluster
+  const auto publish = [&](const Stats& st, int index, int lanes) {
     if (kGrad == 0 && ++ahead > buf.size / 2) {
       ok = ok && warp_wait(&x.coef_full[read.i], read.parity);
       read.next();
     }
-    if (ok && lane < parts) {
-      const int to = (buf.i * parts + rank) * kParts + index;
-      if (parts == 1) {
-        x.part[to] = make_float4(st.m, st.s, st.u, 0.f);
-        tc::mbar_arrive(&x.part_full[buf.i]);
-      } else {
-        st_async(&x.part[to], &x.part_full[buf.i], uint32_t(lane), st.m, st.s, st.u);
-      }
+    if (parts == 1) {
+      if (ok && lane < lanes) x.part[buf.i * row_parts + index + lane] = make_float4(st.m, st.s, st.u, 0.f);
+      __syncwarp();
+      if (ok && lane == 0) tc::mbar_arrive(&x.part_full[buf.i]);
+    } else if (ok && lane < parts) {
+      st_async(&x.part[buf.i * row_parts + rank * (kRoleWarps + kMarkers) + index], &x.part_full[buf.i], uint32_t(lane),
+               st.m, st.s, st.u);
     }
     buf.next();
   };
@@ -1005,7 +1014,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
         const uint32_t src = ring + uint32_t(slot.i * kChunk + tid) * 16u;
         const int left = sh.count - at - tid;
         uint4 v[kPer];
-        if (left >= kChunk) {
+        if (sh.count - at >= kChunk) {
 #pragma unroll
           for (int i = 0; i < kPer; ++i) v[i] = lds16(src + i * kRoleThreads * 16);
         } else {
@@ -1025,7 +1034,10 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
         if (kGrad == 0) free_chunk(&x.empty[slot.i], v, &x.sink[warp]);  // nobody else reads the chunk
         add_vectors<T, kPer, !kDistill>(st, v, a);
       }
-      publish(merge_warp<!kDistill>(st, a), warp);
+      if (parts == 1)
+        publish(merge_warp<!kDistill, kPartLanes>(st, a), warp * kPartLanes, kPartLanes);
+      else
+        publish(merge_warp<!kDistill>(st, a), warp, 1);
     }
   } else if (warp < kControlWarp) {
     // --------------------------------------------------------------------------------------------- gradient
@@ -1112,7 +1124,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           const PolicyIn in = policy_inputs(t, row.row);
           ok = wait_cluster(&x.part_full[buf.i], buf.parity);
           if (!ok) break;
-          const Stats st = merge_parts<true>(x.part + buf.i * parts * kParts, parts * kParts, a);
+          const Stats st = merge_parts<true>(x.part + buf.i * row_parts, row_parts, a);
           o = finish_row<true, kGrad>(a, t, in, row.row, row.label, zy, st, write);
         } else {
           ok = warp_wait(&x.teacher_full[teach.i], teach.parity);
@@ -1127,7 +1139,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           }
           ok = wait_cluster(&x.part_full[buf.i], buf.parity);
           if (!ok) break;
-          const Stats st = merge_parts<false>(x.part + buf.i * parts * kParts, parts * kParts, a);
+          const Stats st = merge_parts<false>(x.part + buf.i * row_parts, row_parts, a);
           float kl = 0.f;
           const float ls = logf(st.s + st.u);
 #pragma unroll
@@ -1327,7 +1339,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           x.twice[teach.i] = again;
           tc::mbar_arrive(&x.row_done[teach.i]);
         }
-        publish(merge_warp<false>(st, a), kRoleWarps);
+        publish(merge_warp<false>(st, a), parts == 1 ? kRoleWarps * kPartLanes : kRoleWarps, 1);
         teach.next();
       }
     } else if (kGrad != 0) {
