@@ -421,34 +421,34 @@ struct RowCoef {
   float c, total, sum;
 };
 
-// From a row's statistics: its outputs (written where `write` is set) and the coefficients of its gradient.
+// From a row's statistics: the coefficients of its gradient (to `ready` as soon as they are known), then its outputs
+// (written where `write` is set).
 //   log q_j = ln 2 d_j - log s,   entropy H = -sum q log q = log s - ln 2 (sum e d) / s,
 //   dz_j = (w / T) (dl/dlogp (1[j = y] - q_j) + c_H q_j (log q_j + H)).
-template <bool kEntropy, int kGrad>
+template <bool kEntropy, int kGrad, typename F>
 __device__ __forceinline__ RowCoef finish_row(const LossRows& a, const PolicyTerms& t, const PolicyIn& in, int64_t r,
-                                              int y, float zy, const Stats& st, bool write) {
+                                              int y, float zy, const Stats& st, bool write, F ready) {
   // products rounded on their own, so that calls with and without a gradient give the same bits
   const float dy = __fmul_rn(zy - st.m, a.k), ls = logf(st.s);
   const float logp = over_t(a, zy - st.m, -ls);
+  RowCoef o{st.m, 0.f, 0.f, 0.f, -1, 0.f, 0.f, 0.f};
+  const float H = kEntropy ? fmaf(-kLn2, st.u / st.s, ls) : 0.f;
+  const PolicyRow p = t.row_loss ? policy_row(t, in, logp, H) : PolicyRow{};
+  if (kGrad != 0 && p.w != 0.f) {
+    const float c = p.dlogp * a.inv_t, h = kGrad == 2 ? p.w * t.entropy_coef * a.inv_t : 0.f;
+    o.y = y;
+    o.A = kGrad == 2 ? (h * (H - ls) - c) / st.s : -c / st.s;
+    o.B = h * kLn2 / st.s;
+    o.at_label = fmaf(ex2(dy), kGrad == 2 ? fmaf(o.B, fmaxf(dy, -1000.f), o.A) : o.A, c);
+  }
+  ready(o);
   if (write) {
     a.logps[r] = logp;
     if (a.stats) a.stats[2 * r] = st.m, a.stats[2 * r + 1] = st.s;
     if (a.coef_zero) zero_coef(a, r);
-  }
-  RowCoef o{st.m, 0.f, 0.f, 0.f, -1, 0.f, 0.f, 0.f};
-  if (!t.row_loss) return o;
-  const float H = kEntropy ? fmaf(-kLn2, st.u / st.s, ls) : 0.f;
-  const PolicyRow p = policy_row(t, in, logp, H);
-  if (write) {
-    t.row_loss[r] = p.loss;
+    if (t.row_loss) t.row_loss[r] = p.loss;
     if (t.entropy) t.entropy[r] = H;
   }
-  if (kGrad == 0 || p.w == 0.f) return o;
-  const float c = p.dlogp * a.inv_t, h = kGrad == 2 ? p.w * t.entropy_coef * a.inv_t : 0.f;
-  o.y = y;
-  o.A = kGrad == 2 ? (h * (H - ls) - c) / st.s : -c / st.s;
-  o.B = h * kLn2 / st.s;
-  o.at_label = fmaf(ex2(dy), kGrad == 2 ? fmaf(o.B, fmaxf(dy, -1000.f), o.A) : o.A, c);
   return o;
 }
 
@@ -480,29 +480,36 @@ __device__ __forceinline__ float mass_at(const int* ids, const float* lp, int K,
   return p;
 }
 
-// From the student's mass outside the ids (st.s) and at them (st.u), the teacher's mass at them (-1: it has no id) and
-// the divergence over them: the row's outputs and the coefficients of its gradient.  With P = sum p and, where the rest is
-// a class of its own, p_r = 1 - P and q_r the student's rest,
+// From the student's mass outside the ids (st.s) and at them (st.u) and the teacher's mass at them (-1: it has no id): the
+// coefficients of the row's gradient.  With P = sum p and, where the rest is a class of its own, p_r = 1 - P and q_r the
+// student's rest,
 //   dz_j = w T ((P + p_r) q_j - p_j) at an id,   w T (P + p_r - p_r / q_r) q_j elsewhere.
 // Where the student has nothing left, a rest of the size of the sum's rounding is none.
-__device__ __forceinline__ RowCoef finish_distill_row(const LossRows& a, const DistillTerms& t, int64_t r, float mass,
-                                                      float weight, float kl, const Stats& st, bool write) {
+struct Rest {
+  float p, q;
+};
+__device__ __forceinline__ Rest rest_of(const DistillTerms& t, float mass, const Stats& st) {
+  Rest o{t.lse ? fmaxf(1.f - mass, 0.f) : 0.f, st.s / (st.s + st.u)};
+  if (o.q == 0.f && o.p < 0x1p-20f) o.p = 0.f;
+  return o;
+}
+__device__ __forceinline__ RowCoef distill_coef(const LossRows& a, float mass, float weight, const Rest& rest,
+                                                const Stats& st) {
   RowCoef o{st.m, 0.f, 0.f, 0.f, -1, 0.f, 0.f, 0.f};
   o.sum = st.s + st.u;
-  const float qr = st.s / o.sum;
-  float pr = t.lse ? fmaxf(1.f - mass, 0.f) : 0.f;
-  if (qr == 0.f && pr < 0x1p-20f) pr = 0.f;
-  if (pr > 0.f) kl += pr * (logf(pr) - logf(qr));
-  if (write) {
-    t.divergence[r] = mass < 0.f ? 0.f : kl;
-    t.row_loss[r] = mass < 0.f || weight == 0.f ? 0.f : weight * t.t2 * kl;
-  }
   if (mass < 0.f || weight == 0.f) return o;
   o.y = 0;
   o.c = weight * float(a.temperature);
-  o.total = mass + pr;
-  o.A = o.c * (o.total - (pr > 0.f && qr != 0.f ? pr / qr : 0.f)) / o.sum;
+  o.total = mass + rest.p;
+  o.A = o.c * (o.total - (rest.p > 0.f && rest.q != 0.f ? rest.p / rest.q : 0.f)) / o.sum;
   return o;
+}
+// ... and, with the divergence over the ids, its outputs
+__device__ __forceinline__ void write_distill_row(const DistillTerms& t, int64_t r, float mass, float weight, float kl,
+                                                  const Rest& rest) {
+  if (rest.p > 0.f) kl += rest.p * (logf(rest.p) - logf(rest.q));
+  t.divergence[r] = mass < 0.f ? 0.f : kl;
+  t.row_loss[r] = mass < 0.f || weight == 0.f ? 0.f : weight * t.t2 * kl;
 }
 
 // One warp: a row's teacher entries (K <= 32 N), lane + 32 i a lane: ids (-1: none) and log-probabilities; returns the sum
@@ -646,7 +653,7 @@ __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
   if (t.row_loss && !t.weights && !t.scale) in.w = mean_of_few(a, nullptr, 0);
   if (parts > 1) tc::cluster_wait();  // every CTA of the cluster runs: their shared memory may be written
   st = merge_rows<NT, kEntropy>(st, a, rank, parts);
-  const RowCoef o = finish_row<kEntropy, kGrad>(a, t, in, r, int(y), zy, st, first);
+  const RowCoef o = finish_row<kEntropy, kGrad>(a, t, in, r, int(y), zy, st, first, [](const RowCoef&) {});
   if constexpr (kGrad != 0) {
     if (o.y < 0) {
       w.template zero<NT>(tid);
@@ -960,7 +967,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
     }
     if (tid >= 16 && tid < 16 + kTeachers) {
       tc::mbar_init(&x.teacher_full[tid - 16], 1);
-      tc::mbar_init(&x.teacher_free[tid - 16], 1);
+      tc::mbar_init(&x.teacher_free[tid - 16], kGrad ? 2 : 1);  // control and patcher
       tc::mbar_init(&x.row_done[tid - 16], kRoleWarps + 1);
     }
     if (tid >= 32) {
@@ -1117,7 +1124,12 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
         continue;
       }
       if (mine) {
-        RowCoef o;
+        const auto ready = [&](const RowCoef& o) {
+          if (lane != 0) return;
+          if (parts > 1) tc::mbar_arrive_expect_tx(&x.part_full[buf.i], part_bytes);  // for its next use
+          x.coef[buf.i] = o;
+          tc::mbar_arrive(&x.coef_full[buf.i]);
+        };
         if constexpr (!kDistill) {
           // asked for while the row's statistics are still being formed
           const float zy = to_f32((logits + row.row * a.ld)[row.label]);
@@ -1125,7 +1137,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           ok = wait_cluster(&x.part_full[buf.i], buf.parity);
           if (!ok) break;
           const Stats st = merge_parts<true>(x.part + buf.i * row_parts, row_parts, a);
-          o = finish_row<true, kGrad>(a, t, in, row.row, row.label, zy, st, write);
+          finish_row<true, kGrad>(a, t, in, row.row, row.label, zy, st, write, ready);
         } else {
           ok = warp_wait(&x.teacher_full[teach.i], teach.parity);
           if (!ok) break;
@@ -1140,6 +1152,8 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           ok = wait_cluster(&x.part_full[buf.i], buf.parity);
           if (!ok) break;
           const Stats st = merge_parts<false>(x.part + buf.i * row_parts, row_parts, a);
+          const Rest rest = rest_of(t, mass, st);
+          ready(distill_coef(a, mass, wt, rest, st));
           float kl = 0.f;
           const float ls = logf(st.s + st.u);
 #pragma unroll
@@ -1148,16 +1162,9 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
             if (k >= t.K || te.id[k] < 0) continue;
             kl = distill_term(a, kl, te.lp[k], zk[i], st.m, ls);
           }
-          o = finish_distill_row(a, t, row.row, mass, wt, warp_sum(kl), st, write);
-          if (kGrad == 0) {
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&x.teacher_free[teach.i]);
-          }
-        }
-        if (parts > 1 && lane == 0) tc::mbar_arrive_expect_tx(&x.part_full[buf.i], part_bytes);  // for its next use
-        if (lane == 0) {
-          x.coef[buf.i] = o;
-          tc::mbar_arrive(&x.coef_full[buf.i]);
+          kl = warp_sum(kl);  // needs every lane's entries: the teacher's buffer is handed back after it
+          if (lane == 0) tc::mbar_arrive(&x.teacher_free[teach.i]);
+          if (write) write_distill_row(t, row.row, mass, wt, kl, rest);
         }
       }
       buf.next();
