@@ -1597,49 +1597,82 @@ __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* part, int64
   if (threadIdx.x == 0) *loss = float(v * factor);
 }
 
-// One CTA per pair (sequences 2p chosen, 2p + 1 rejected): the log ratios of both, the pair's loss, and
-// d loss / d logp of their tokens.  The CTA that is done last adds the pairs' losses, in the pairs' order.
-__global__ void __launch_bounds__(kSmall) pair_kernel(LossRows a, PairTerms t) {
-  await_previous();
-  __shared__ double red[kSmall / 32];
+// One CTA per pair (sequences 2p chosen, 2p + 1 rejected; half of the threads each): the log ratios of both, the pair's
+// loss, and d loss / d logp of their tokens.  The CTA that is done last adds the pairs' losses, in the pairs' order.
+// What bounds it is one chain of loads: offsets, labels, logits.  None of them is of the forward kernel's making, so a
+// thread's first kAhead tokens are looked up while that one still runs, and only the statistics are waited for.
+constexpr int kPairThreads = 512, kAhead = 4;
+__global__ void __launch_bounds__(kPairThreads) pair_kernel(LossRows a, PairTerms t) {
+  constexpr int kHalf = kPairThreads / 2, kHalfWarps = kHalf / 32;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ double red[kPairThreads / 32];
+  __shared__ int live[kPairThreads / 32];
   const int64_t p = blockIdx.x;
-  int64_t lo[2], hi[2];
+  const int side = int(threadIdx.x) / kHalf, tid = int(threadIdx.x) % kHalf;
+  int64_t lo = t.cu[2 * p + side], hi = t.cu[2 * p + side + 1];
+  const bool outside = lo < 0 || hi > a.n || hi < lo;  // offsets out of range: the sequence counts as empty
+  if (outside) lo = hi = 0;
+  const double inv_t = 1.0 / a.temperature;
+  // a token: whether it counts, and its logit less the reference's log-probability
+  int count = 0;
+  struct Token {
+    double z, ref;
+    bool use;
+  };
+  const auto token = [&](int64_t r) {
+    Token k{0.0, 0.0, false};
+    const int64_t y = ld_index(a.labels, a.index_dtype, r);
+    if (y == a.ignore_index) return k;
+    ++count;
+    if (y < 0 || y >= a.V) return k;  // recorded by the forward kernel
+    k.use = true;
+    k.z = double(ld_as_f32(a.logits, a.dtype, r * a.ld + y));
+    k.ref = t.ref ? double(t.ref[r]) : 0.0;
+    return k;
+  };
+  // from the row's statistics, and not from its log-probability in fp32: a log ratio is a sum of differences of near values
+  const auto ratio = [&](const Token& k, int64_t r) {
+    return (k.z - double(a.stats[2 * r])) * inv_t - log(double(a.stats[2 * r + 1])) - k.ref;
+  };
+  Token ahead[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int64_t r = lo + tid + i * kHalf;
+    ahead[i] = r < hi ? token(r) : Token{0.0, 0.0, false};
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (outside && tid == 0) record_device_error(&g_loss_error, kErrSlotOutOfRange);
+  double v = 0.0;
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (ahead[i].use) v += ratio(ahead[i], lo + tid + i * kHalf);
+  for (int64_t r = lo + tid + kAhead * kHalf; r < hi; r += kHalf) {
+    const Token k = token(r);
+    if (k.use) v += ratio(k, r);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  count = __reduce_add_sync(0xffffffffu, count);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v, live[threadIdx.x >> 5] = count;
+  __syncthreads();
   double sum[2], cnt[2];
   for (int i = 0; i < 2; ++i) {
-    lo[i] = t.cu[2 * p + i];
-    hi[i] = t.cu[2 * p + i + 1];
-    if (lo[i] < 0 || hi[i] > a.n || hi[i] < lo[i]) {  // offsets out of range: the sequence counts as empty
-      if (threadIdx.x == 0) record_device_error(&g_loss_error, kErrSlotOutOfRange);
-      lo[i] = hi[i] = 0;
-    }
-    double v = 0.0, c = 0.0;
-    for (int64_t r = lo[i] + threadIdx.x; r < hi[i]; r += kSmall) {
-      const int64_t y = ld_index(a.labels, a.index_dtype, r);
-      if (y == a.ignore_index) continue;
-      c += 1.0;
-      if (y < 0 || y >= a.V) continue;  // recorded by the forward kernel
-      // from the row's statistics, and not from its log-probability in fp32: a log ratio is a sum of differences of near
-      // values
-      const double z = double(ld_as_f32(a.logits, a.dtype, r * a.ld + y)), m = double(a.stats[2 * r]);
-      v += (z - m) / a.temperature - log(double(a.stats[2 * r + 1])) - (t.ref ? double(t.ref[r]) : 0.0);
-    }
-    sum[i] = block_sum_f64(v, red);
-    cnt[i] = t.normalise ? fmax(block_sum_f64(c, red), 1.0) : 1.0;
-    sum[i] /= cnt[i];
+    double sv = 0.0;
+    int sc = 0;
+    for (int w = 0; w < kHalfWarps; ++w) sv += red[i * kHalfWarps + w], sc += live[i * kHalfWarps + w];
+    cnt[i] = t.normalise ? fmax(double(sc), 1.0) : 1.0;
+    sum[i] = sv / cnt[i];
   }
-  const double h = double(t.beta) * (sum[0] - sum[1]);
-  // log sigmoid(h) = min(h, 0) - log1p(e^-|h|)
-  const double l1p = log1p(exp(-fabs(h)));
-  const double eps = double(t.smoothing);
-  const double dh = 1.0 / (1.0 + exp(-h)) - (1.0 - eps);
+  const double h = double(t.beta) * (sum[0] - sum[1]), eps = double(t.smoothing);
+  const double e = exp(-fabs(h));  // sigmoid(h) = 1 / (1 + e^-h), without an overflow
+  const double dh = (h < 0.0 ? e : 1.0) / (1.0 + e) - (1.0 - eps);
+  const float c = float((side == 0 ? dh : -dh) * double(t.beta) / (double(t.pairs) * cnt[side]));
+  for (int64_t r = lo + tid; r < hi; r += kHalf) t.coef[r] = c;
   if (threadIdx.x == 0) {
+    const double l1p = log1p(e);  // log sigmoid(h) = min(h, 0) - log1p(e^-|h|)
     t.log_ratios[2 * p] = float(sum[0]);
     t.log_ratios[2 * p + 1] = float(sum[1]);
     t.pair_loss[p] = float(-((1.0 - eps) * (fmin(h, 0.0) - l1p) + eps * (fmin(-h, 0.0) - l1p)));
-  }
-  for (int i = 0; i < 2; ++i) {
-    const float c = float((i == 0 ? dh : -dh) * double(t.beta) / (double(t.pairs) * cnt[i]));
-    for (int64_t r = lo[i] + threadIdx.x; r < hi[i]; r += kSmall) t.coef[r] = c;
   }
   __shared__ bool last;
   if (threadIdx.x == 0) {
@@ -1649,8 +1682,8 @@ __global__ void __launch_bounds__(kSmall) pair_kernel(LossRows a, PairTerms t) {
   }
   __syncthreads();
   if (!last) return;
-  double v = 0.0;
-  for (int64_t q = threadIdx.x; q < t.pairs; q += kSmall) v += double(__ldcg(t.pair_loss + q));
+  v = 0.0;
+  for (int64_t q = threadIdx.x; q < t.pairs; q += kPairThreads) v += double(__ldcg(t.pair_loss + q));
   v = block_sum_f64(v, red);
   if (threadIdx.x == 0) *t.loss = float(v / double(t.pairs));
 }
@@ -1866,7 +1899,7 @@ cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, cudaSt
   cudaError_t e = a.n > 0 ? launch_logp(f, PolicyTerms{}, false, stream)
                           : cudaMemsetAsync(t.pairs_done, 0, sizeof(unsigned), stream);
   if (e != cudaSuccess) return e;
-  e = launch(pair_kernel, t.pairs, kSmall, 1, 0, a.n > 0, stream, a, t);
+  e = launch(pair_kernel, t.pairs, kPairThreads, 1, 0, a.n > 0, stream, a, t);
   if (e != cudaSuccess || !a.dlogits || a.n == 0) return e;
   return launch_token_logprobs_backward(a, t.coef, true, stream);
 }
