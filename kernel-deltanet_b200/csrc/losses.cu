@@ -8,15 +8,15 @@
 // lose nothing to a large m.  Exponentials are taken to base 2: e^{(z - m)/T} = 2^{(z - m) k}, k = log2(e) / T,
 // with ex2.approx (2 ulp).  The difference is formed before the product: a fused z k - m k would leave the
 // rounding of m k at z = m (a lone entry's log-probability would not be 0) and overflow at the type's lowest
-// value.  Where every logit of a row is
-// -inf (or one is NaN or +inf) the row's results are NaN, as the formula gives.
+// value.  Where every logit of a row is -inf (or one is NaN or +inf) the row's results are NaN, as the formula gives.
 //
 // Two kinds of kernels.  In the first a row belongs to a warp, a CTA or a cluster of up to 8 CTAs, each with a
-// contiguous share of the row's 16-byte vectors.  A share of up to 8 vectors a thread stays in registers between the two
-// passes over it (statistics, then gradient), so the logits are read from memory once and the gradient is written once;
-// the row's statistics are merged through warp shuffles, one barrier, and (in a cluster) one exchange through
+// contiguous share of the row's 16-byte vectors.  A share of up to 8 vectors a thread stays in registers between the
+// two passes over it (statistics, then gradient), so the logits are read from memory once and the gradient is written
+// once; the row's statistics are merged through warp shuffles, one barrier, and (in a cluster) one exchange through
 // distributed shared memory.  Longer shares are taken in rounds and read again for the gradient.  The second, for the
-// losses with a gradient over many long rows, streams them through a ring in shared memory: loss_stream_kernel.
+// losses of a policy or a teacher over many long rows, streams them through a ring in shared memory:
+// loss_stream_kernel.
 #include <math.h>
 
 #include <algorithm>
@@ -76,8 +76,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
-// First thing in the kernels of a call that makes several launches: the next kernel of the same call may be launched (it waits in turn, its launch
-// overlaps this one's end), and the previous one's results are awaited (at once where it was launched without overlap).
+// First thing in the kernels of a call that makes several launches: the next kernel of the same call may be launched
+// (it waits in turn, its launch overlaps this one's end), and the previous one's results are awaited (at once where it
+// was launched without overlap).  Worth 1 to 2 us a launch.
 __device__ __forceinline__ void await_previous() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -268,8 +269,8 @@ struct Cta {
   }
 };
 
-// x / T + c in fp32, rounded once: the quotient's two halves (see LossRows; not through log2(e) / T or one rounded 1 / T,
-// whose error would show in a log-probability)
+// x / T + c in fp32, rounded once: the quotient's two halves (see LossRows; not through log2(e) / T or one rounded
+// 1 / T, whose error would show in a log-probability)
 __device__ __forceinline__ float over_t(const LossRows& a, float x, float c) {
   return fmaf(x, a.inv_hi, fmaf(x, a.inv_lo, c));
 }
@@ -480,9 +481,9 @@ __device__ __forceinline__ float mass_at(const int* ids, const float* lp, int K,
   return p;
 }
 
-// From the student's mass outside the ids (st.s) and at them (st.u) and the teacher's mass at them (-1: it has no id): the
-// coefficients of the row's gradient.  With P = sum p and, where the rest is a class of its own, p_r = 1 - P and q_r the
-// student's rest,
+// From the student's mass outside the ids (st.s) and at them (st.u) and the teacher's mass at them (-1: it has no id):
+// the coefficients of the row's gradient.  With P = sum p and, where the rest is a class of its own, p_r = 1 - P and
+// q_r the student's rest,
 //   dz_j = w T ((P + p_r) q_j - p_j) at an id,   w T (P + p_r - p_r / q_r) q_j elsewhere.
 // Where the student has nothing left, a rest of the size of the sum's rounding is none.
 struct Rest {
@@ -512,8 +513,8 @@ __device__ __forceinline__ void write_distill_row(const DistillTerms& t, int64_t
   t.row_loss[r] = mass < 0.f || weight == 0.f ? 0.f : weight * t.t2 * kl;
 }
 
-// One warp: a row's teacher entries (K <= 32 N), lane + 32 i a lane: ids (-1: none) and log-probabilities; returns the sum
-// of the probabilities, -1 without an id.
+// One warp: a row's teacher entries (K <= 32 N), lane + 32 i a lane: ids (-1: none) and log-probabilities; returns the
+// sum of the probabilities, -1 without an id.
 template <int N>
 __device__ __forceinline__ float teacher_probabilities(const LossRows& a, const DistillTerms& t, int64_t r, bool record,
                                                        int (&id)[N], float (&lp)[N]) {
@@ -579,8 +580,8 @@ __device__ __forceinline__ void add_at(float2* g, int e, float c) {
   }
 }
 
-// log2(e) / T in two halves: with one, its rounding moves every exponent of a row the same way, and the log of the row's
-// sum by as much as 1e-6.
+// log2(e) / T in two halves: with one, its rounding moves every exponent of a row the same way, and the log of the
+// row's sum by as much as 1e-6.
 struct Log2Scale {
   float hi, lo;
 };
@@ -610,13 +611,19 @@ __device__ __forceinline__ void add_vectors(Stats& st, const uint4* v, const Los
   const float m = fmaxf(st.m, Vec<T>::template largest<N>(v));
   rescale<kMoment>(st, m, a);
   float s, u;
-  accumulate<T, N, kMoment>(v, m == -INFINITY ? 0.f : m, Log2Scale{a.k_hi, a.k_lo}, s, u);  // without a finite logit: 2^-inf each
+  const float base = m == -INFINITY ? 0.f : m;  // without a finite logit: 2^-inf each
+  accumulate<T, N, kMoment>(v, base, Log2Scale{a.k_hi, a.k_lo}, s, u);
   st.s += s;
   st.u += u;
 }
 
 // -------------------------------------------------------------------- token log-probabilities, policy loss
 // kEntropy: the row's entropy is formed; kGrad: the gradient is (kGrad == 2: with the entropy's term).
+// Without a gradient the memory bounds it: bf16 8192 x 32000, 7168 rows that count, 459 MB read in 81 us, 86 % of the
+// measured copy rate (CTAs of 128 threads at different places of their rows; what is missing is the last round of
+// them).  With one, a CTA that keeps its row in registers loads, computes and stores by turns, and the SM's few CTAs
+// run in step: 600 x 32000 26 us, 45 % of the rate of one read and one write; many long rows are the streaming
+// kernel's.
 template <typename T, int NT, bool kEntropy, int kGrad>
 __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
     logp_kernel(LossRows a, PolicyTerms t, int parts) {
@@ -675,7 +682,9 @@ __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
   }
 }
 
-// d/dz of sum_t dlogps_t logp_t from the saved statistics: one read, one write, nothing to reduce
+// d/dz of sum_t dlogps_t logp_t from the saved statistics: one read, one write, nothing to reduce.  Bound by memory:
+// 8192 x 32000 bf16 in 165 us, 97 % of the measured copy rate.  (Loading a row before the coefficients are awaited made
+// a call of 8192 x 32000 slower, 239 us against 221: every CTA then waits for its coefficient behind its loads.)
 template <typename T, int NT>
 __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
     logp_backward_kernel(LossRows a, const float* dlogps, int parts) {
@@ -722,15 +731,23 @@ __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
 //   marker     (distillation only) adds up the exponentials at the teacher's ids in every chunk that arrives and puts
 //              -inf in their place, so that what the statistics role sums is the student's mass outside the ids (one
 //              minus the mass inside would lose it when that is near one);
-//   statistics (8 warps) maximum and sums of every chunk as it arrives, then one partial result a warp (in a cluster,
-//              to the shared memory of every CTA of it);
-//   control    (2 warps, row about) merges a row's partials, computes the loss, writes the row's outputs and
-//              publishes the coefficients of its gradient;
+//   statistics (8 warps) maximum and sums of every chunk as it arrives, then a warp's partial results: 8 for the policy
+//              loss, whose control warps have the time to add them up, else one; in a cluster, one to the shared memory
+//              of every CTA of it;
+//   control    (2 warps, row about) merges a row's partials, publishes the coefficients of its gradient, and then
+//              computes and writes the row's outputs;
 //   gradient   (8 warps) reads the row's chunks once more from shared memory, writes the gradient, frees them;
 //   patcher    (distillation only) writes the gradient's entries at the ids once the row's gradient is written.
 // A slot's, a row's and a buffer's barriers are waited for by each role at every use and in order: a wait by parity
 // cannot tell a use from the one two before.  Every wait is bounded; after one that gave up a role ends,
 // kErrLossWaitTimeout is recorded, and the CTA returns when its copies have landed.
+//
+// What bounds it: bf16 rows of 32000, 3.4 us a row and SM for the policy loss against 2.9 us of memory (7168 of 8192
+// rows of 131072, two CTAs a row: 742 us, 83 % of the measured copy rate of one read and one write; fp32 32000 with a
+// teacher's 64 entries: 5.9 us a row, 98 %).  The statistics warps are busy for 5600 of a row's 6900 cycles; a row
+// stays in the ring until its gradient is written, and the ring holds three of 64 KB, so the time from a row's last
+// chunk to its coefficients counts in full.  Other shapes of the ring and the roles, the same policy loss: 256 threads
+// x 4 vectors 748 us (kept); x 3 828, x 2 867, x 5 810, x 6 817; 320 threads x 3 813, 384 x 3 833, 384 x 2 815.
 constexpr int kPer = 4;                // vectors that a thread of a role takes at a time
 constexpr int kBuf = 8;                // rows between a partial result and its use, see Exchange
 constexpr int kQueue = 32;             // rows between the producer and the last of the other roles
@@ -766,15 +783,16 @@ struct Teacher {
   int id[kMaxTop];
 };
 
-// What the roles pass on.  Rows that count use the buffers for partial results and coefficients in turn, 16 of them,
-// or 8 in a cluster.  They are free when they are written: with a gradient, the ring holds 13 rows at most (3 in a
-// cluster, where a share is more than 4 chunks), a row leaves it when its coefficients have been used, and another
-// CTA's control is at most that far behind its statistics; without, statistics (and the marker) wait for the control
-// warps to be at most half of the buffers behind.  The teachers' buffers are handed back by a barrier.
+// What the roles pass on.  Rows that count use the 8 buffers for partial results and coefficients in turn.  They are
+// free when they are written.  With a gradient, a row leaves the ring when its coefficients have been used, and when
+// the last chunk of a row is there the ring holds nothing older than the 6 rows before it (a share is 2 chunks or
+// more), in a cluster than the 2 rows before it (more than 4 chunks), where another CTA's control is then at most 6
+// rows behind.  Without one, statistics (and the marker) wait for the control warps to be at most half of the buffers
+// behind.  The teachers' buffers are handed back by a barrier.
 template <bool kDistill>
 struct Exchange {
   uint4 response;                                                  // of a request for more rows
-  // (m, s, u) of the statistics warps (of a few lanes of each, or one for each of every CTA of a cluster) and the marker
+  // (m, s, u) of the statistics warps (kPartLanes of each, or one for each of every CTA of a cluster) and the marker
   float4 part[kBuf * kMaxCluster * (kRoleWarps + kDistill)];
   QueuedRow queue[kQueue];
   RowCoef coef[kBuf];
@@ -882,8 +900,8 @@ struct RowShare {
   }
 };
 
-// Hands a chunk back once the warp's loads of it have returned.  An arrival does not wait for loads that are still under
-// way (it overtook them: the next copy was then read in their place); the store of a word that needs all of them does.
+// Hands a chunk back once the warp's loads of it have returned.  An arrival does not wait for loads still under way
+// (it overtook them: the next copy was then read in their place); the store of a word that needs all of them does.
 template <int N>
 __device__ __forceinline__ void free_chunk(uint64_t* bar, const uint4 (&v)[N], uint32_t* sink) {
   uint32_t all = 0u;
@@ -993,7 +1011,8 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
   Place buf(kBuf), slot(kSlots), teach(kTeachers);
   Place read(buf.size);  // half of the buffers behind buf
   int ahead = 0;
-  // a warp's partial results of the row (statistics warps, then the marker): lanes [0, lanes), or to every CTA of the cluster
+  // a warp's partial results of the row (statistics warps, then the marker): lanes [0, lanes), or the warp's one to
+  // every CTA of the cluster
   const auto publish = [&](const Stats& st, int index, int lanes) {
     if (kGrad == 0 && ++ahead > buf.size / 2) {
       ok = ok && warp_wait(&x.coef_full[read.i], read.parity);
@@ -1395,7 +1414,9 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
 // ------------------------------------------------------------------------------------------- distillation
 // Teacher entries are held in shared memory; a bit per element of the share marks the teacher's ids, so that the
 // student's mass outside them is a sum of its own (one minus the mass inside would lose what is left when that is
-// near one).  The gradient is written densely, then the entries at the ids are written over.
+// near one).  The gradient is written densely, then the entries at the ids are written over.  For few rows, short rows
+// and more than 128 entries: 16 x 32000 bf16 with 32 entries 9 us, the latency of one row (teacher, statistics, merge,
+// gradient one after another); 4096 x 32000 with 64 entries 155 us, where the streaming kernel takes 124.
 template <typename T, int NT, bool kTail, bool kGrad>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, DistillTerms t, int parts) {
   extern __shared__ float sm[];
@@ -1571,6 +1592,7 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
   return v;
 }
 
+// The two sums over rows, one CTA each (a fixed order): latency, 2 to 3 us after the kernel before them.
 // scale = 1 / (rows that count): rows whose label is not ignore_index, or (K > 0) whose first id is >= 0
 __global__ void __launch_bounds__(1024) live_scale_kernel(const void* __restrict__ labels, int index_dtype, int64_t n,
                                                           int64_t stride, bool by_sign, int64_t ignore_index,
@@ -1630,7 +1652,8 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(LossRows a, PairTerm
     k.ref = t.ref ? double(t.ref[r]) : 0.0;
     return k;
   };
-  // from the row's statistics, and not from its log-probability in fp32: a log ratio is a sum of differences of near values
+  // from the row's statistics, and not from its log-probability in fp32: a log ratio is a sum of differences of near
+  // values
   const auto ratio = [&](const Token& k, int64_t r) {
     return (k.z - double(a.stats[2 * r])) * inv_t - log(double(a.stats[2 * r + 1])) - k.ref;
   };
@@ -1688,14 +1711,34 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(LossRows a, PairTerm
   if (threadIdx.x == 0) *t.loss = float(v / double(t.pairs));
 }
 
-// x *= *scale, row by row; nothing is read or written where the scale is one
-template <typename T>
-__global__ void __launch_bounds__(kSmall) scale_kernel(T* __restrict__ x, int64_t ld, int64_t n, int64_t V,
-                                                         const float* __restrict__ scale) {
+// x *= *scale; nothing is read or written where the scale is one, which is the common case (so the grid is small, and
+// its CTAs take share after share of a row: a warp 256 vectors, or 256 threads 2048).  One read, one write, bound by
+// memory: 8192 x 32000 bf16 in 165 us, 97 % of the measured copy rate.  A bf16 gradient is rounded a second time here.
+template <typename T, int NT>
+__global__ void __launch_bounds__(kSmall) scale_kernel(LossRows a, const float* __restrict__ scale, int parts) {
+  constexpr int kUnits = kSmall / NT;  // shares of a CTA
   const float f = *scale;
   if (f == 1.f) return;
-  for (int64_t r = blockIdx.x; r < n; r += gridDim.x)
-    for (int64_t j = threadIdx.x; j < V; j += kSmall) from_f32(x + r * ld + j, to_f32(x[r * ld + j]) * f);
+  const int tid = int(threadIdx.x) % NT;
+  for (int64_t u = int64_t(blockIdx.x) * kUnits + threadIdx.x / NT; u < a.n * parts; u += int64_t(gridDim.x) * kUnits) {
+    const Share<T> w(a, u / parts, int(u % parts), parts);
+    for (int at = w.v0 + tid; at < w.v1; at += NT * kNV) {
+      uint4 v[kNV];
+#pragma unroll
+      for (int i = 0; i < kNV; ++i)
+        if (const int vi = at + i * NT; vi < w.v1)  // (not through the read-only path: it is written here)
+          v[i] = w.whole(vi) ? *reinterpret_cast<const uint4*>(w.dz + (vi * w.E - w.off))
+                             : load_edge(w.z, vi * w.E - w.off, w.V);
+#pragma unroll
+      for (int i = 0; i < kNV; ++i) {
+        if (at + i * NT >= w.v1) break;
+        float2 g[Vec<T>::E / 2];
+#pragma unroll
+        for (int j = 0; j < Vec<T>::E / 2; ++j) g[j] = mul2(Vec<T>::minus(v[i], j, 0.f), make_float2(f, f));
+        w.store(at + i * NT, g);
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------- launches
@@ -1724,9 +1767,9 @@ Split choose_split(const LossRows& a) {
 }
 
 // Log-probabilities alone read a row once and keep nothing of it: where there are rows enough, small CTAs in as many
-// rounds as it takes (at different places of their rows, those of an SM keep the memory busy).  B200, bf16: 16384 x 4096
-// 26 us with a warp a row, 53 with 128 threads; 4096 x 32000 47 us with 128 threads, 65 with the row in the registers of
-// 512; 2400 x 131072 101 us with 256 threads, 107 with 128, 326 with a cluster of four times 512.
+// rounds as it takes (at different places of their rows, those of an SM keep the memory busy).  B200, bf16:
+// 16384 x 4096 26 us with a warp a row, 53 with 128 threads; 4096 x 32000 47 us with 128 threads, 65 with the row in
+// the registers of 512; 2400 x 131072 101 us with 256 threads, 107 with 128, 326 with a cluster of four times 512.
 Split choose_scan_split(const LossRows& a) {
   if (a.n < 2 * current_sm_count()) return choose_split(a);
   const int64_t vecs = row_vectors(a);
@@ -1855,7 +1898,9 @@ cudaError_t launch_distill(const LossRows& a, const DistillTerms& t, bool after,
   return dispatch(a, s, [&](auto z, auto nt) {
     using T = decltype(z);
     constexpr int NT = decltype(nt)::value < 128 ? 128 : decltype(nt)::value;
-    const auto go = [&](auto kernel) { return launch_rows(kernel, a.n, s, true, size_t(t.K) * 8, after, stream, a, t); };
+    const auto go = [&](auto kernel) {
+      return launch_rows(kernel, a.n, s, true, size_t(t.K) * 8, after, stream, a, t);
+    };
     if (t.lse) return a.dlogits ? go(distill_kernel<T, NT, true, true>) : go(distill_kernel<T, NT, true, false>);
     return a.dlogits ? go(distill_kernel<T, NT, false, true>) : go(distill_kernel<T, NT, false, false>);
   });
@@ -1883,8 +1928,8 @@ cudaError_t launch_policy_loss(const LossRows& a, PolicyTerms t, float* loss, cu
   if (t.weights || a.n <= kFewRows) t.scale = nullptr;  // few rows: their own kernel counts
   const bool mean = t.scale != nullptr;
   if (mean) {
-    const cudaError_t e = launch(live_scale_kernel, 1, 1024, 1, 0, false, stream, a.labels, a.index_dtype, a.n, 1, false,
-                                 a.ignore_index, const_cast<float*>(t.scale));
+    const cudaError_t e = launch(live_scale_kernel, 1, 1024, 1, 0, false, stream, a.labels, a.index_dtype, a.n, 1,
+                                 false, a.ignore_index, const_cast<float*>(t.scale));
     if (e != cudaSuccess) return e;
   }
   if (cudaError_t e = launch_logp(a, t, mean, stream); e != cudaSuccess) return e;
@@ -1918,12 +1963,21 @@ cudaError_t launch_distillation_loss(const LossRows& a, DistillTerms t, float* l
 
 cudaError_t launch_scale_rows(void* x, int dtype, int64_t ld, int64_t n, int64_t V, const float* scale,
                               cudaStream_t stream) {
-  const unsigned grid = unsigned(n < 148 * 8 ? n : 148 * 8);
+  LossRows a = {};
+  a.logits = a.dlogits = x;
+  a.dtype = dtype;
+  a.ld = a.ld_d = ld;
+  a.n = n;
+  a.V = V;
+  // a warp a share for short rows: 16384 x 1000 bf16 10 us, 35 with 256 threads
+  const int64_t vecs = row_vectors(a), threads = vecs <= 512 ? 32 : kSmall;
+  const int parts = int((vecs + threads * kNV - 1) / (threads * kNV));
+  const int64_t units = kSmall / threads;
+  const int64_t grid = std::min<int64_t>((n * parts + units - 1) / units, 8 * current_sm_count());
+  const auto go = [&](auto kernel) { return launch(kernel, grid, kSmall, 1, 0, false, stream, a, scale, parts); };
   if (dtype == KDN_DTYPE_BF16)
-    scale_kernel<__nv_bfloat16><<<grid, kSmall, 0, stream>>>(static_cast<__nv_bfloat16*>(x), ld, n, V, scale);
-  else
-    scale_kernel<float><<<grid, kSmall, 0, stream>>>(static_cast<float*>(x), ld, n, V, scale);
-  return cudaGetLastError();
+    return threads == 32 ? go(scale_kernel<__nv_bfloat16, 32>) : go(scale_kernel<__nv_bfloat16, kSmall>);
+  return threads == 32 ? go(scale_kernel<float, 32>) : go(scale_kernel<float, kSmall>);
 }
 
 cudaError_t loss_read_error(cudaStream_t stream, int* code) {

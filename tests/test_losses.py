@@ -664,3 +664,23 @@ def test_gradients_against_differences():
             slope = (_np(g) * d).sum()
             # |d| ~ 1 an element and |g| summed over a row at most 2 |coef|: 100 eps in all
             assert abs(_differences(f, z64, d) - slope) <= 100 * _eps(z, 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,ld", [(1, 1, 1), (3, 2, 2), (5, 7, 16), (67, 1000, 1000), (2500, 130, 131), (9, 4099, 4099),
+                                    (33, 20011, 20016), (3, 70001, 70001)])
+def test_gradients_scaled_in_place(n, V, ld, dtype):
+    """The factor of an upstream gradient: one product in fp32, rounded once; what lies beside the rows stays."""
+    from kdn_b200 import _lib
+
+    lib = _lib.load()
+    gen = torch.Generator(device="cuda").manual_seed(n + V)
+    x = torch.randn(n, ld, device="cuda", generator=gen).to(dtype)
+    for factor in (1.0, 2.5, 0.0, -0.125):
+        want, got = x.clone(), x.clone()
+        want[:, :V] = (x[:, :V].float() * factor).to(dtype)
+        scale = torch.tensor(factor, device="cuda")
+        assert lib.kdn_scale_rows(got.data_ptr(), _lib.dtype_code(got), ld, n, V, scale.data_ptr(),
+                                  torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(got, want), factor
