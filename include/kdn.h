@@ -350,9 +350,9 @@ int kdn_varlen_causal_attention(const void* q, const void* k_cache, const void* 
  * Losses over vocabulary logits (no reference entry points; the reference trains with torch's losses, and upcycles a
  * teacher's layers in pipeline/transmute.py).  logits [n, V] (dtype KDN_DTYPE_F32 or KDN_DTYPE_BF16), rows ld elements
  * apart (ld >= V, any ld and any element-aligned start; rows of one 16-byte phase move by vectors).  x = logits /
- * temperature (in [1e-6, 1e6]), log q = x - log sum e^x; sums and statistics are fp32.  dlogits (same dtype, rows ld_d apart; must not
- * overlap logits) is the gradient of the loss, rounded once; NULL: no gradient is formed.  logits equal to -inf have
- * probability zero; a row of nothing else, or with a NaN or +inf, gives NaN.
+ * temperature (in [1e-6, 1e6]), log q = x - log sum e^x; sums and statistics are fp32.  dlogits (same dtype, rows ld_d
+ * apart; must not overlap logits) is the gradient of the loss, rounded once; NULL: no gradient is formed.  logits equal
+ * to -inf have probability zero; a row of nothing else, or with a NaN or +inf, gives NaN.
  *
  * A row whose label is ignore_index counts for nothing: its logits are not read, its outputs and its gradient row are
  * zero.  A label outside [0, V) is treated the same way and recorded for kdn_device_error (code 1).  weights [n] fp32

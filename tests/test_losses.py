@@ -668,8 +668,8 @@ def test_gradients_against_differences():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,V,ld", [(1, 1, 1), (3, 2, 2), (5, 7, 16), (67, 1000, 1000), (2500, 130, 131), (9, 4099, 4099),
-                                    (33, 20011, 20016), (3, 70001, 70001)])
+@pytest.mark.parametrize("n,V,ld", [(1, 1, 1), (3, 2, 2), (5, 7, 16), (67, 1000, 1000), (2500, 130, 131),
+                                    (9, 4099, 4099), (33, 20011, 20016), (3, 70001, 70001)])
 def test_gradients_scaled_in_place(n, V, ld, dtype):
     """The factor of an upstream gradient: one product in fp32, rounded once; what lies beside the rows stays."""
     from kdn_b200 import _lib
