@@ -684,3 +684,30 @@ def test_gradients_scaled_in_place(n, V, ld, dtype):
         assert lib.kdn_scale_rows(got.data_ptr(), _lib.dtype_code(got), ld, n, V, scale.data_ptr(),
                                   torch.cuda.current_stream().cuda_stream) == 0
         assert torch.equal(got, want), factor
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,V", [(16, 4100), (600, 32000)])
+def test_losses_replayed_from_a_graph(n, V):
+    import kdn_b200 as kdn
+
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    z = torch.randn(n, V, device="cuda", generator=gen).to(torch.bfloat16)
+    y = torch.randint(V, (n,), device="cuda", generator=gen)
+    old, adv = (torch.randn(n, device="cuda", generator=gen) for _ in range(2))
+    ids = torch.randint(V, (n, 33), device="cuda", generator=gen)
+    top = torch.randn(n, 33, device="cuda", generator=gen)
+    cu = torch.tensor([0, n // 4, n // 2, n // 2 + 3, n], device="cuda")
+    calls = [lambda: (kdn.token_logprobs(z, y),), lambda: kdn.policy_loss_and_grad(z, y, old, adv, ref_logps=old),
+             lambda: kdn.preference_loss_and_grad(z, y, cu), lambda: kdn.distillation_loss_and_grad(z, top, ids)]
+    for call in calls:
+        want = [t.clone() for t in call()]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = call()
+        for _ in range(2):
+            for t in got:
+                t.fill_(-1)
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(want, got))
