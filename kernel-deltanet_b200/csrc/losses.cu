@@ -370,7 +370,8 @@ struct PolicyRow {
 // The clipped policy loss of one token: r = e^(logp - old),
 //   l = -min(r A, clip(r, 1 - lo, 1 + hi) A) + c_kl (e^g - 1 - g) - c_H H,   g = ref - logp,
 // where e^g - 1 - g >= 0 estimates KL(policy || reference) from the policy's own sample.  The gradient of the
-// first term is -r A where the unclipped product is the smaller (or the two are equal), else zero.
+// first term is -r A where the unclipped product is the smaller (or the two are equal), else zero.  A NaN in either
+// product is NaN in the loss and in the gradient (so no fminf or fmaxf here: they return their other argument).
 struct PolicyIn {
   float w, adv, old, ref;
 };
@@ -383,9 +384,11 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, const Poli
   PolicyRow p;
   p.w = in.w;
   const float adv = in.adv, ratio = expf(logp - in.old);
-  const float free = ratio * adv, clipped = fminf(fmaxf(ratio, 1.f - t.clip_low), 1.f + t.clip_high) * adv;
-  float l = free <= clipped ? -free : -clipped;
-  float d = free <= clipped ? -free : 0.f;
+  const float lo = 1.f - t.clip_low, hi = 1.f + t.clip_high;
+  const float clipped = (ratio < lo ? lo : ratio > hi ? hi : ratio) * adv;
+  const float free = adv == 0.f ? clipped : ratio * adv;  // zero, too, where the ratio has overflowed
+  float l = free > clipped ? -clipped : -free;
+  float d = free > clipped ? 0.f : -free;
   if (t.ref_logps) {
     const float g = in.ref - logp, em = expm1f(g);
     l = fmaf(t.kl_coef, em - g, l);

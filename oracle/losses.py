@@ -53,7 +53,7 @@ def policy_loss(logits, actions, old_logps, advantages, ref_logps=None, weights=
         a = np.asarray(advantages, np.float64)
         free, clipped = r * a, np.clip(r, 1.0 - clip_low, 1.0 + clip_high) * a
         each = -np.minimum(free, clipped) - entropy_coef * H
-        slope = -np.where(free <= clipped, free, 0.0)
+        slope = -np.where(free > clipped, 0.0, free)  # NaN where free is
         if ref_logps is not None and kl_coef:
             g = np.asarray(ref_logps, np.float64) - logps
             each = each + kl_coef * (np.expm1(g) - g)
