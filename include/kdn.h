@@ -374,8 +374,9 @@ int kdn_varlen_causal_attention(const void* q, const void* k_cache, const void* 
  *     negative ids are padding, and a row whose FIRST id is negative counts for nothing; an id >= V is skipped and
  *     recorded, code 1; an id given twice counts twice).  teacher_lse NULL: p = softmax of the row's entries / T; else
  *     p = e^(teacher / T - teacher_lse[t]) (log-sum-exp of the teacher's whole row / T) and what is left of the
- *     teacher's mass, 1 - sum p, is compared with the student's mass outside the ids as one more class (where the
- *     student has none the divergence is +inf and the gradient outside the ids zero).
+ *     teacher's mass, 1 - sum p, is compared with the student's mass outside the ids as one more class, however far below
+ *     the ids' its logits lie (where all of them are -inf the divergence is +inf and the gradient outside the ids zero;
+ *     where that mass is below 2^-126, a 1 - sum p below 2^-20 is rounding and counts as zero).
  *     divergence[t] = KL(p || q), loss = T^2 sum_t w_t divergence[t].
  *   kdn_scale_rows: x *= *scale in place (a device scalar); returns without touching x when it is 1.
  * Workspaces: the *_workspace_size entries, 256-byte aligned.

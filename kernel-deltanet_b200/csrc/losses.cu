@@ -202,6 +202,18 @@ __device__ __noinline__ uint4 mask_edge(uint4 v, int j0, int V) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+// a vector whose elements of a set bit become -inf
+template <typename T>
+__device__ __forceinline__ uint4 mask_bits(uint4 v, uint32_t bits) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t m = sizeof(T) == 4 ? 0u - (bits >> i & 1u)
+                                      : (bits >> 2 * i & 1u) * 0xffffu + (bits >> (2 * i + 1) & 1u) * 0xffff0000u;
+    w[i] = (w[i] & ~m) | (Vec<T>::kFill & m);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 template <typename T>
 __device__ __noinline__ void store_edge(T* dz, uint4 v, int j0, int V) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -275,24 +287,62 @@ __device__ __forceinline__ float over_t(const LossRows& a, float x, float c) {
   return fmaf(x, a.inv_hi, fmaf(x, a.inv_lo, c));
 }
 
-// Largest logit m, sum of exponentials below it, and a second sum (see its use) of a part of a row.
+// Largest logit m of a part of a row, the sum s of exponentials below it and (kMoment) u = sum e^d d (base 2), which a
+// change of m shifts.
+template <bool kMoment>
 struct Stats {
-  float m, s, u;
+  float m = -INFINITY, s = 0.f;
+};
+template <>
+struct Stats<true> {
+  float m = -INFINITY, s = 0.f, u = 0.f;
+};
+using Sum = Stats<false>;
+
+// The distillation loss: the logits outside the teacher's ids and those at them, each below its own largest.  A
+// student's mass outside the ids may lie so far below the row's largest logit that every exponential relative to that is
+// zero, while its logarithm and an entry's share of it are ordinary numbers.
+struct Apart {
+  Sum out, in;
 };
 
-// The statistics of two parts together.  kMoment: u is sum e^d d (base 2), which a change of m shifts; else a sum
-// like s.  A part without a finite logit has m = -inf and sums of zero (or NaN) and is left as it is.
-// (The factor is expf's, which errs to both sides; ex2.approx truncates, and a sum is rescaled several times.)
-template <bool kMoment>
-__device__ __forceinline__ void rescale(Stats& a, float m, const LossRows& r) {
+// Statistics relative to another largest logit.  A part without a finite logit has m = -inf and sums of zero (or NaN)
+// and is left as it is.  (The factor is expf's, which errs to both sides; ex2.approx truncates, and a sum is rescaled
+// several times.)
+__device__ __forceinline__ void rescale(Stats<true>& a, float m, const LossRows& r) {
   if (a.m == m) return;
   const float d = (a.m - m) * r.k, f = expf(over_t(r, a.m - m, 0.f));
-  if constexpr (kMoment)
-    a.u = f == 0.f ? 0.f : f * fmaf(a.s, d, a.u);
-  else
-    a.u *= f;
+  a.u = f == 0.f ? 0.f : f * fmaf(a.s, d, a.u);
   a.s *= f;
   a.m = m;
+}
+__device__ __forceinline__ void rescale(Sum& a, float m, const LossRows& r) {
+  if (a.m == m) return;
+  a.s *= expf(over_t(r, a.m - m, 0.f));
+  a.m = m;
+}
+
+// a and b together
+template <bool kMoment>
+__device__ __forceinline__ void add(Stats<kMoment>& a, Stats<kMoment> b, const LossRows& r) {
+  const float m = fmaxf(a.m, b.m);
+  rescale(a, m, r);
+  rescale(b, m, r);
+  a.s += b.s;
+  if constexpr (kMoment) a.u += b.u;
+}
+__device__ __forceinline__ void add(Apart& a, const Apart& b, const LossRows& r) {
+  add(a.out, b.out, r);
+  add(a.in, b.in, r);
+}
+
+__device__ __forceinline__ float4 pack(const Stats<true>& a) { return make_float4(a.m, a.s, a.u, 0.f); }
+__device__ __forceinline__ float4 pack(const Sum& a) { return make_float4(a.m, a.s, 0.f, 0.f); }
+__device__ __forceinline__ float4 pack(const Apart& a) { return make_float4(a.out.m, a.out.s, a.in.m, a.in.s); }
+__device__ __forceinline__ void unpack(const float4& t, Stats<true>& a) { a.m = t.x, a.s = t.y, a.u = t.z; }
+__device__ __forceinline__ void unpack(const float4& t, Sum& a) { a.m = t.x, a.s = t.y; }
+__device__ __forceinline__ void unpack(const float4& t, Apart& a) {
+  a.out.m = t.x, a.out.s = t.y, a.in.m = t.z, a.in.s = t.w;
 }
 
 // the largest of a warp's values (none is NaN), in the order of their bits as integers
@@ -303,50 +353,59 @@ __device__ __forceinline__ float warp_max(float x) {
 }
 
 // the statistics of a warp's lanes together; kLeft > 1: of lanes of equal index modulo kLeft, about the warp's maximum
-template <bool kMoment, int kLeft = 1>
-__device__ __forceinline__ Stats merge_warp(Stats a, const LossRows& r) {
-  rescale<kMoment>(a, warp_max(a.m), r);
+template <int kLeft = 1, bool kMoment>
+__device__ __forceinline__ Stats<kMoment> merge_warp(Stats<kMoment> a, const LossRows& r) {
+  rescale(a, warp_max(a.m), r);
 #pragma unroll
   for (int o = 16; o >= kLeft; o >>= 1) {
     a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
-    a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+    if constexpr (kMoment) a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+  }
+  return a;
+}
+__device__ __forceinline__ Apart merge_warp(Apart a, const LossRows& r) {
+  const float out = warp_max(a.out.m), in = warp_max(a.in.m);
+  rescale(a.out, out, r);
+  rescale(a.in, in, r);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.out.s += __shfl_xor_sync(0xffffffffu, a.out.s, o);
+    a.in.s += __shfl_xor_sync(0xffffffffu, a.in.s, o);
   }
   return a;
 }
 
 // ... of `count` parts in shared memory, by every warp that asks
-template <bool kMoment>
-__device__ __forceinline__ Stats merge_parts(const float4* p, int count, const LossRows& r) {
+template <typename S>
+__device__ __forceinline__ S merge_parts(const float4* p, int count, const LossRows& r) {
   const int lane = threadIdx.x & 31;
-  Stats a{-INFINITY, 0.f, 0.f};
-  for (int i = lane; i < count; i += 32) {
-    const float4 t = p[i];
-    Stats b{t.x, t.y, t.z};
-    const float m = fmaxf(a.m, b.m);
-    rescale<kMoment>(a, m, r);
-    rescale<kMoment>(b, m, r);
-    a.s += b.s;
-    a.u += b.u;
+  S a, b;
+  if (lane < count) unpack(p[lane], a);
+  for (int i = lane + 32; i < count; i += 32) {
+    unpack(p[i], b);
+    add(a, b, r);
   }
-  return merge_warp<kMoment>(a, r);
+  return merge_warp(a, r);
 }
 
 // ... of all threads of the row's cluster
-template <int NT, bool kMoment>
-__device__ __forceinline__ Stats merge_rows(Stats a, const LossRows& r, int rank, int parts) {
-  a = merge_warp<kMoment>(a, r);
+template <int NT, typename S>
+__device__ __forceinline__ S merge_rows(S a, const LossRows& r, int rank, int parts) {
+  a = merge_warp(a, r);
   if constexpr (NT == 32) return a;
   __shared__ float4 part[NT / 32];
   __shared__ float4 remote[kMaxCluster];
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float4(a.m, a.s, a.u, 0.f);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = pack(a);
   __syncthreads();
-  a = merge_parts<kMoment>(part, NT / 32, r);
+  a = merge_parts<S>(part, NT / 32, r);
   if (parts > 1) {
-    if (threadIdx.x < unsigned(parts))
-      tc::st_cluster_v4(tc::mapa(tc::smem_u32(&remote[rank]), threadIdx.x), a.m, a.s, a.u, 0.f);
+    if (threadIdx.x < unsigned(parts)) {
+      const float4 t = pack(a);
+      tc::st_cluster_v4(tc::mapa(tc::smem_u32(&remote[rank]), threadIdx.x), t.x, t.y, t.z, t.w);
+    }
     tc::cluster_arrive();
     tc::cluster_wait();
-    a = merge_parts<kMoment>(remote, parts, r);
+    a = merge_parts<S>(remote, parts, r);
   }
   return a;
 }
@@ -418,11 +477,11 @@ __device__ __forceinline__ void zero_coef(const LossRows& a, int64_t r) {
 }
 
 // What the gradient of a row needs: dz_j = 2^d (A + B d) with d = (z_j - m) k, and dz_y; for the distillation loss the
-// entries at the teacher's ids are c (total q - p), q = 2^d / sum.
+// entries at the teacher's ids are c (total q - p), q = 2^((z_j - top) k) / sum.
 struct RowCoef {
   float m, A, B, at_label;
   int y;  // -1: the gradient is zero
-  float c, total, sum;
+  float c, total, top, sum;
 };
 
 // From a row's statistics: the coefficients of its gradient (to `ready` as soon as they are known), then its outputs
@@ -431,12 +490,13 @@ struct RowCoef {
 //   dz_j = (w / T) (dl/dlogp (1[j = y] - q_j) + c_H q_j (log q_j + H)).
 template <bool kEntropy, int kGrad, typename F>
 __device__ __forceinline__ RowCoef finish_row(const LossRows& a, const PolicyTerms& t, const PolicyIn& in, int64_t r,
-                                              int y, float zy, const Stats& st, bool write, F ready) {
+                                              int y, float zy, const Stats<kEntropy>& st, bool write, F ready) {
   // products rounded on their own, so that calls with and without a gradient give the same bits
   const float dy = __fmul_rn(zy - st.m, a.k), ls = logf(st.s);
   const float logp = over_t(a, zy - st.m, -ls);
-  RowCoef o{st.m, 0.f, 0.f, 0.f, -1, 0.f, 0.f, 0.f};
-  const float H = kEntropy ? fmaf(-kLn2, st.u / st.s, ls) : 0.f;
+  RowCoef o{st.m, 0.f, 0.f, 0.f, -1, 0.f, 0.f, 0.f, 0.f};
+  float H = 0.f;
+  if constexpr (kEntropy) H = fmaf(-kLn2, st.u / st.s, ls);
   const PolicyRow p = t.row_loss ? policy_row(t, in, logp, H) : PolicyRow{};
   if (kGrad != 0 && p.w != 0.f) {
     const float c = p.dlogp * a.inv_t, h = kGrad == 2 ? p.w * t.entropy_coef * a.inv_t : 0.f;
@@ -484,34 +544,41 @@ __device__ __forceinline__ float mass_at(const int* ids, const float* lp, int K,
   return p;
 }
 
-// From the student's mass outside the ids (st.s) and at them (st.u) and the teacher's mass at them (-1: it has no id):
-// the coefficients of the row's gradient.  With P = sum p and, where the rest is a class of its own, p_r = 1 - P and
-// q_r the student's rest,
-//   dz_j = w T ((P + p_r) q_j - p_j) at an id,   w T (P + p_r - p_r / q_r) q_j elsewhere.
-// Where the student has nothing left, a rest of the size of the sum's rounding is none.
+// The row's softmax from the student's sums outside the ids and at them, and what is left of the teacher: p_r = 1 - P,
+// P = sum p, where the rest is a class of its own (else zero).  Where the student has nothing left, or less than an fp32
+// number of the row's own scale could hold (q_r < 2^-126), a p_r of the size of P's rounding is none: times log q_r it
+// would be any number.
 struct Rest {
-  float p, q;
+  float m, sum;  // the row's largest logit, its sum of exponentials below that
+  float f;       // e^((largest outside - m) / T)
+  float p;
 };
-__device__ __forceinline__ Rest rest_of(const DistillTerms& t, float mass, const Stats& st) {
-  Rest o{t.lse ? fmaxf(1.f - mass, 0.f) : 0.f, st.s / (st.s + st.u)};
-  if (o.q == 0.f && o.p < 0x1p-20f) o.p = 0.f;
+__device__ __forceinline__ Rest rest_of(const LossRows& a, bool tail, float mass, const Apart& st) {
+  Rest o;
+  o.m = fmaxf(st.out.m, st.in.m);
+  o.f = expf(over_t(a, st.out.m - o.m, 0.f));
+  o.sum = fmaf(st.out.s, o.f, st.in.s * expf(over_t(a, st.in.m - o.m, 0.f)));
+  o.p = tail ? fmaxf(1.f - mass, 0.f) : 0.f;
+  if (o.p > 0.f && o.p < 0x1p-20f && st.out.s * o.f < 0x1p-126f * o.sum) o.p = 0.f;
   return o;
 }
+// The coefficients of the row's gradient (mass < 0: the teacher has no id),
+//   dz_j = w T ((P + p_r) q_j - p_j) at an id,   w T ((P + p_r) q_j - p_r q_j / q_r) elsewhere,
+// where q_j / q_r is taken below the largest logit outside the ids.  (No logit there: the gradient there is zero.)
 __device__ __forceinline__ RowCoef distill_coef(const LossRows& a, float mass, float weight, const Rest& rest,
-                                                const Stats& st) {
-  RowCoef o{st.m, 0.f, 0.f, 0.f, -1, 0.f, 0.f, 0.f};
-  o.sum = st.s + st.u;
+                                                const Apart& st) {
+  RowCoef o{st.out.s == 0.f ? rest.m : st.out.m, 0.f, 0.f, 0.f, -1, 0.f, 0.f, rest.m, rest.sum};
   if (mass < 0.f || weight == 0.f) return o;
   o.y = 0;
   o.c = weight * float(a.temperature);
   o.total = mass + rest.p;
-  o.A = o.c * (o.total - (rest.p > 0.f && rest.q != 0.f ? rest.p / rest.q : 0.f)) / o.sum;
+  o.A = o.c * (o.total * rest.f / rest.sum - (rest.p > 0.f && st.out.s != 0.f ? rest.p / st.out.s : 0.f));
   return o;
 }
-// ... and, with the divergence over the ids, its outputs
-__device__ __forceinline__ void write_distill_row(const DistillTerms& t, int64_t r, float mass, float weight, float kl,
-                                                  const Rest& rest) {
-  if (rest.p > 0.f) kl += rest.p * (logf(rest.p) - logf(rest.q));
+// ... and, with the divergence over the ids, its outputs (ls: the log of the row's sum)
+__device__ __forceinline__ void write_distill_row(const LossRows& a, const DistillTerms& t, int64_t r, float mass,
+                                                  float weight, float kl, const Rest& rest, const Apart& st, float ls) {
+  if (rest.p > 0.f) kl += rest.p * (logf(rest.p) - over_t(a, st.out.m - rest.m, logf(st.out.s) - ls));
   t.divergence[r] = mass < 0.f ? 0.f : kl;
   t.row_loss[r] = mass < 0.f || weight == 0.f ? 0.f : weight * t.t2 * kl;
 }
@@ -610,14 +677,14 @@ __device__ __forceinline__ void accumulate(const uint4* v, float base, Log2Scale
 
 // `st` with N more vectors
 template <typename T, int N, bool kMoment>
-__device__ __forceinline__ void add_vectors(Stats& st, const uint4* v, const LossRows& a) {
+__device__ __forceinline__ void add_vectors(Stats<kMoment>& st, const uint4* v, const LossRows& a) {
   const float m = fmaxf(st.m, Vec<T>::template largest<N>(v));
-  rescale<kMoment>(st, m, a);
+  rescale(st, m, a);
   float s, u;
   const float base = m == -INFINITY ? 0.f : m;  // without a finite logit: 2^-inf each
   accumulate<T, N, kMoment>(v, base, Log2Scale{a.k_hi, a.k_lo}, s, u);
   st.s += s;
-  st.u += u;
+  if constexpr (kMoment) st.u += u;
 }
 
 // -------------------------------------------------------------------- token log-probabilities, policy loss
@@ -655,14 +722,14 @@ __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
     }
   };
   const int rounds = max(1, (w.v1 - w.v0 + NT * kNV - 1) / (NT * kNV));
-  Stats st{-INFINITY, 0.f, 0.f};
+  Stats<kEntropy> st;
   for (int q = 0; q < rounds; ++q) {
     load(w.v0 + q * NT * kNV);
-    add_vectors<T, kNV, kEntropy>(st, v, a);
+    add_vectors<T, kNV>(st, v, a);
   }
   if (t.row_loss && !t.weights && !t.scale) in.w = mean_of_few(a, nullptr, 0);
   if (parts > 1) tc::cluster_wait();  // every CTA of the cluster runs: their shared memory may be written
-  st = merge_rows<NT, kEntropy>(st, a, rank, parts);
+  st = merge_rows<NT>(st, a, rank, parts);
   const RowCoef o = finish_row<kEntropy, kGrad>(a, t, in, r, int(y), zy, st, first, [](const RowCoef&) {});
   if constexpr (kGrad != 0) {
     if (o.y < 0) {
@@ -795,7 +862,7 @@ struct Teacher {
 template <bool kDistill>
 struct Exchange {
   uint4 response;                                                  // of a request for more rows
-  // (m, s, u) of the statistics warps (kPartLanes of each, or one for each of every CTA of a cluster) and the marker
+  // packed sums of the statistics warps (kPartLanes of each, or one for each of every CTA of a cluster) and the marker
   float4 part[kBuf * kMaxCluster * (kRoleWarps + kDistill)];
   QueuedRow queue[kQueue];
   RowCoef coef[kBuf];
@@ -849,10 +916,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
 }
 
 // 16 bytes to the same place of CTA `rank` of the cluster, counted by the barrier of that CTA
-__device__ __forceinline__ void st_async(float4* p, uint64_t* bar, uint32_t rank, float a, float b, float c) {
+__device__ __forceinline__ void st_async(float4* p, uint64_t* bar, uint32_t rank, const float4& t) {
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
                    tc::mapa(tc::smem_u32(p), rank)),
-               "f"(a), "f"(b), "f"(c), "f"(0.f), "r"(tc::mapa(tc::smem_u32(bar), rank))
+               "f"(t.x), "f"(t.y), "f"(t.z), "f"(t.w), "r"(tc::mapa(tc::smem_u32(bar), rank))
                : "memory");
 }
 
@@ -1016,18 +1083,18 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
   int ahead = 0;
   // a warp's partial results of the row (statistics warps, then the marker): lanes [0, lanes), or the warp's one to
   // every CTA of the cluster
-  const auto publish = [&](const Stats& st, int index, int lanes) {
+  const auto publish = [&](const float4& sums, int index, int lanes) {
     if (kGrad == 0 && ++ahead > buf.size / 2) {
       ok = ok && warp_wait(&x.coef_full[read.i], read.parity);
       read.next();
     }
     if (parts == 1) {
-      if (ok && lane < lanes) x.part[buf.i * row_parts + index + lane] = make_float4(st.m, st.s, st.u, 0.f);
+      if (ok && lane < lanes) x.part[buf.i * row_parts + index + lane] = sums;
       __syncwarp();
       if (ok && lane == 0) tc::mbar_arrive(&x.part_full[buf.i]);
     } else if (ok && lane < parts) {
       st_async(&x.part[buf.i * row_parts + rank * (kRoleWarps + kMarkers) + index], &x.part_full[buf.i], uint32_t(lane),
-               st.m, st.s, st.u);
+               sums);
     }
     buf.next();
   };
@@ -1037,7 +1104,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
     while ((ok = ok && reader.next(x, row)) && row.row >= 0) {
       if (row.label < 0) continue;
       const RowShare<T> sh(logits + row.row * a.ld, V, per, rank);
-      Stats st{-INFINITY, 0.f, 0.f};
+      Stats<!kDistill> st;
       for (int at = 0; at < sh.count && ok; at += kChunk, slot.next()) {
         ok = warp_wait(kDistill ? &x.marked[slot.i] : &x.full[slot.i], slot.parity);
         const uint32_t src = ring + uint32_t(slot.i * kChunk + tid) * 16u;
@@ -1061,12 +1128,18 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           }
         }
         if (kGrad == 0) free_chunk(&x.empty[slot.i], v, &x.sink[warp]);  // nobody else reads the chunk
-        add_vectors<T, kPer, !kDistill>(st, v, a);
+        add_vectors<T, kPer>(st, v, a);
       }
+      const auto sums = [](const Stats<!kDistill>& t) {
+        if constexpr (kDistill)
+          return pack(Apart{t, Sum{}});
+        else
+          return pack(t);
+      };
       if (parts == 1)
-        publish(merge_warp<!kDistill, kPartLanes>(st, a), warp * kPartLanes, kPartLanes);
+        publish(sums(merge_warp<kPartLanes>(st, a)), warp * kPartLanes, kPartLanes);
       else
-        publish(merge_warp<!kDistill>(st, a), warp, 1);
+        publish(sums(merge_warp(st, a)), warp, 1);
     }
   } else if (warp < kControlWarp) {
     // --------------------------------------------------------------------------------------------- gradient
@@ -1158,7 +1231,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           const PolicyIn in = policy_inputs(t, row.row);
           ok = wait_cluster(&x.part_full[buf.i], buf.parity);
           if (!ok) break;
-          const Stats st = merge_parts<true>(x.part + buf.i * row_parts, row_parts, a);
+          const auto st = merge_parts<Stats<true>>(x.part + buf.i * row_parts, row_parts, a);
           finish_row<true, kGrad>(a, t, in, row.row, row.label, zy, st, write, ready);
         } else {
           ok = warp_wait(&x.teacher_full[teach.i], teach.parity);
@@ -1173,20 +1246,20 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           }
           ok = wait_cluster(&x.part_full[buf.i], buf.parity);
           if (!ok) break;
-          const Stats st = merge_parts<false>(x.part + buf.i * row_parts, row_parts, a);
-          const Rest rest = rest_of(t, mass, st);
+          const Apart st = merge_parts<Apart>(x.part + buf.i * row_parts, row_parts, a);
+          const Rest rest = rest_of(a, t.lse != nullptr, mass, st);
           ready(distill_coef(a, mass, wt, rest, st));
           float kl = 0.f;
-          const float ls = logf(st.s + st.u);
+          const float ls = logf(rest.sum);
 #pragma unroll
           for (int i = 0; i < kMaxTop / 32; ++i) {
             const int k = lane + 32 * i;
             if (k >= t.K || te.id[k] < 0) continue;
-            kl = distill_term(a, kl, te.lp[k], zk[i], st.m, ls);
+            kl = distill_term(a, kl, te.lp[k], zk[i], rest.m, ls);
           }
           kl = warp_sum(kl);  // needs every lane's entries: the teacher's buffer is handed back after it
           if (lane == 0) tc::mbar_arrive(&x.teacher_free[teach.i]);
-          if (write) write_distill_row(t, row.row, mass, wt, kl, rest);
+          if (write) write_distill_row(a, t, row.row, mass, wt, kl, rest, st, ls);
         }
       }
       buf.next();
@@ -1317,7 +1390,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < kMaxTop / 32; ++i) id[i] = x.teacher[teach.i].id[lane + 32 * i];
         const RowShare<T> sh(logits + row.row * a.ld, V, per, rank);
-        Stats st{-INFINITY, 0.f, 0.f};
+        Sum st;
         bool again = false;
         for (int at = 0; at < sh.count && ok; at += kChunk, slot.next()) {
           ok = warp_wait(&x.full[slot.i], slot.parity);
@@ -1355,10 +1428,10 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
               here[i] = here[i] && own && bits_to_f32<T>(bits[i]) != -INFINITY;
               if (here[i]) m = fmaxf(m, bits_to_f32<T>(bits[i]));
             }
-            rescale<false>(st, m, a);
+            rescale(st, m, a);
 #pragma unroll
             for (int i = 0; i < kMaxTop / 32; ++i)
-              if (here[i]) st.u += ex2((bits_to_f32<T>(bits[i]) - m) * a.k);
+              if (here[i]) st.s += ex2((bits_to_f32<T>(bits[i]) - m) * a.k);
           } else if (lane == 0) {
             tc::mbar_arrive(&x.marked[slot.i]);
           }
@@ -1368,7 +1441,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           x.twice[teach.i] = again;
           tc::mbar_arrive(&x.row_done[teach.i]);
         }
-        publish(merge_warp<false>(st, a), parts == 1 ? kRoleWarps * kPartLanes : kRoleWarps, 1);
+        publish(pack(Apart{Sum{}, merge_warp(st, a)}), parts == 1 ? kRoleWarps * kPartLanes : kRoleWarps, 1);
         teach.next();
       }
     } else if (kGrad != 0) {
@@ -1397,7 +1470,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
         for (int i = 0; i < kMaxTop / 32; ++i) {
           if (id[i] < 0) continue;
           const float p = twice ? mass_at(te.id, te.lp, t.K, id[i]) : expf(te.lp[lane + 32 * i]);
-          const float q = ex2((zk[i] - o.m) * a.k) / o.sum;
+          const float q = ex2((zk[i] - o.top) * a.k) / o.sum;
           from_f32(static_cast<T*>(a.dlogits) + row.row * a.ld_d + id[i], o.c * fmaf(q, o.total, -p));
         }
         __syncwarp();
@@ -1480,7 +1553,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
     if (lane == 0) ts[0] = ps;
   }
   const int rounds = max(1, (w.v1 - w.v0 + NT * kNV - 1) / (NT * kNV));
-  Stats st{-INFINITY, 0.f, 0.f};  // s: outside the ids (kTail) or everywhere; u: at the ids (kTail)
+  Apart st;  // without kTail: all of the row outside
   for (int q = 0; q < rounds; ++q) {
     const int at = w.v0 + q * NT * kNV;
     if (q > 0) {
@@ -1498,61 +1571,41 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
       if (atomicOr(&mark[vi >> 2], bit) & bit) {
         twice = 1;
       } else if (kTail) {
-        const float zk = to_f32(w.z[id[k]]), m = fmaxf(st.m, zk);
-        rescale<false>(st, m, a);
-        st.u += zk == -INFINITY ? 0.f : ex2((zk - m) * a.k);
+        const float zk = to_f32(w.z[id[k]]), m = fmaxf(st.in.m, zk);
+        rescale(st.in, m, a);
+        st.in.s += zk == -INFINITY ? 0.f : ex2((zk - m) * a.k);
       }
     }
     __syncthreads();
-    const float m = fmaxf(st.m, Vec<T>::template largest<kNV>(v));
-    rescale<false>(st, m, a);
-    const float b = m == -INFINITY ? 0.f : m;
+    if constexpr (kTail) {  // (their entries of the gradient are written over in any case)
 #pragma unroll
-    for (int i = 0; i < kNV; ++i) {
-      float s, u;
-      if constexpr (kTail) {
+      for (int i = 0; i < kNV; ++i) {
         const uint32_t bits = reinterpret_cast<const uint8_t*>(mark)[tid + i * NT];
-        if (bits != 0) {  // a few vectors of a row: element by element
-#pragma unroll
-          for (int e = 0; e < Vec<T>::E; ++e) {
-            const float2 z2 = Vec<T>::pair(v[i], e / 2);
-            const float x = ex2((((e & 1) ? z2.y : z2.x) - b) * a.k);
-            if (!(bits >> e & 1u)) st.s += x;
-          }
-          continue;
-        }
+        if (bits != 0) v[i] = mask_bits<T>(v[i], bits);
       }
-      accumulate<T, 1, false>(v + i, b, Log2Scale{a.k_hi, a.k_lo}, s, u);
-      st.s += s;
     }
+    add_vectors<T, kNV>(st.out, v, a);
   }
   if (parts > 1) tc::cluster_wait();
-  st = merge_rows<NT, false>(st, a, rank, parts);
-  const float S = kTail ? st.s + st.u : st.s, ls = logf(S), ps = ts[0];
-  // what is left of both; where the student has nothing left, a rest of the size of the sum's rounding is none
-  const float qr = kTail ? st.s / S : 1.f;
-  float pr = kTail ? fmaxf(1.f - ps, 0.f) : 0.f;
-  if (qr == 0.f && pr < 0x1p-20f) pr = 0.f;
+  st = merge_rows<NT>(st, a, rank, parts);
+  const float ps = any ? ts[0] : -1.f;
+  const Rest rest = rest_of(a, kTail, ps, st);
   const float wt = t.weights ? t.weights[r] : t.scale ? *t.scale : mean_of_few(a, t.ids, K);
   if (rank == 0 && tid < 32) {
     float kl = 0.f;
+    const float ls = logf(rest.sum);
     for (int k = lane; k < K; k += 32) {
-      if (id[k] >= 0) kl = distill_term(a, kl, tp[k], to_f32(w.z[id[k]]), st.m, ls);
+      if (id[k] >= 0) kl = distill_term(a, kl, tp[k], to_f32(w.z[id[k]]), rest.m, ls);
     }
     kl = warp_sum(kl);
-    if (pr > 0.f) kl += pr * (logf(pr) - logf(qr));
-    if (lane == 0) {
-      t.divergence[r] = any ? kl : 0.f;
-      t.row_loss[r] = any && wt != 0.f ? wt * t.t2 * kl : 0.f;
-    }
+    if (lane == 0) write_distill_row(a, t, r, ps, wt, kl, rest, st, ls);
   }
   if constexpr (kGrad) {
-    if (wt == 0.f || !any) {
+    const RowCoef o = distill_coef(a, ps, wt, rest, st);
+    if (o.y < 0) {
       w.template zero<NT>(tid);
       return;
     }
-    const float c = wt * float(a.temperature), A = ps + pr, R = pr > 0.f && qr != 0.f ? pr / qr : 0.f;
-    const float f = c * (A - R) / S;
     for (int q = rounds - 1; q >= 0; --q) {
       if (q < rounds - 1) load(w.v0 + q * NT * kNV);
 #pragma unroll
@@ -1560,7 +1613,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
         const int vi = w.v0 + q * NT * kNV + tid + i * NT;
         if (vi >= w.v1) break;
         float2 g[Vec<T>::E / 2];
-        vector_grad<T, 1>(v[i], st.m, a.k, f, 0.f, g);
+        vector_grad<T, 1>(v[i], o.m, a.k, o.A, 0.f, g);
         w.store(vi, g);
       }
     }
@@ -1575,8 +1628,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
         for (int i = 0; i < K; ++i)
           if (id[i] == id[k]) P += expf(tp[i]);
       }
-      const float qk = ex2((to_f32(w.z[id[k]]) - st.m) * a.k) / S;
-      from_f32(w.dz + id[k], c * fmaf(qk, A, -P));
+      const float qk = ex2((to_f32(w.z[id[k]]) - o.top) * a.k) / o.sum;
+      from_f32(w.dz + id[k], o.c * fmaf(qk, o.total, -P));
     }
   }
 }

@@ -107,12 +107,12 @@ def distillation_loss(logits, teacher_logits, teacher_ids, teacher_lse=None, wei
         if teacher_lse is not None:
             outside = np.ones(V, bool)
             outside[at] = False
-            p_rest, q_rest = max(0.0, 1.0 - p.sum()), q[outside].sum()
+            p_rest, log_q_rest = max(0.0, 1.0 - p.sum()), np.logaddexp.reduce(lq[outside], initial=-np.inf)
             g = q * (p.sum() + p_rest)
-            if p_rest > 0:
-                with np.errstate(divide="ignore"):
-                    divergence[r] += p_rest * (np.log(p_rest) - np.log(q_rest))
-                    g[outside] -= q[outside] * (p_rest / q_rest)
+            if p_rest > 0:  # the share of an entry in the rest: q / q_rest, which both may be too small for
+                divergence[r] += p_rest * (np.log(p_rest) - log_q_rest)
+                if log_q_rest != -np.inf:
+                    g[outside] -= p_rest * np.exp(lq[outside] - log_q_rest)
         np.add.at(g, at, -p)
         if w[r] != 0.0:
             d[r] = w[r] * temperature * g

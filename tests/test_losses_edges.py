@@ -98,3 +98,128 @@ def test_a_ratio_that_overflows_times_no_advantage_is_nothing():
     want = oracle.policy_loss(_np(z), y, old, adv)
     assert abs(want[0] + 1.2 / 4) < 1e-6 and abs(float(loss) - want[0]) < 1e-6  # the one clipped ratio, 1 + 0.2
     assert not want[3].any() and not d.any()
+
+
+# -------------------------------------------------------------------------------- a student's mass far below its top
+def _rest_reference(z, T, t, ids, lse):
+    """One row in float64, in logarithms throughout: the divergence, p and q at the ids, p_r and log q_r of what is
+    left, log q outside relative to q_r."""
+    lq = z / T - np.logaddexp.reduce(z / T)
+    p = np.exp(t / T - lse)
+    outside = np.ones(z.size, bool)
+    outside[ids] = False
+    p_r, log_qr = max(0.0, 1.0 - p.sum()), np.logaddexp.reduce(lq[outside])
+    kl = (p * (t / T - lse - lq[ids])).sum() + (p_r * (np.log(p_r) - log_qr) if p_r > 0 else 0.0)
+    return kl, p, np.exp(lq[ids]), p_r, log_qr, outside, lq - log_qr
+
+
+def test_oracle_of_a_far_rest():
+    rng = np.random.default_rng(0)
+    n, V, K = 4, 30, 5
+    z = rng.standard_normal((n, V))
+    ids = np.stack([rng.permutation(V)[:K] for _ in range(n)])
+    for r, drop in enumerate((5.0, 300.0, 1e4, 1e6)):
+        outside = np.ones(V, bool)
+        outside[ids[r]] = False
+        z[r, outside] -= drop
+    t = rng.standard_normal((n, K))
+    lse = np.logaddexp.reduce(t, axis=1) + 0.3
+    loss, kl, d = oracle.distillation_loss(z, t, ids, lse)
+    for r in range(n):
+        want, p, q, p_r, log_qr, outside, rel = _rest_reference(z[r], 1.0, t[r], ids[r], lse[r])
+        assert abs(kl[r] - want) <= 1e-12 * abs(want)
+        total = p.sum() + p_r
+        assert np.allclose(d[r][outside] * n, total * np.exp(rel[outside] + log_qr) - p_r * np.exp(rel[outside]), 1e-11, 0)
+        # the divergence moves by -p_r softmax of the outside along them, however far they lie
+        step = np.where(outside, rng.standard_normal(V), 0.0)
+        f = lambda h: oracle.distillation_loss(z[r:r + 1] + h * step, t[r:r + 1], ids[r:r + 1], lse[r:r + 1])[1][0]
+        h = 1e-4
+        assert abs((f(h) - f(-h)) / (2 * h) - (d[r] * n * step).sum()) <= 1e-6 + 1e-15 * abs(want) / h
+
+
+@gpu
+@pytest.mark.parametrize("drop", [20.0, 60.0, 86.5, 87.2, 87.8, 100.0, 1e4])
+@pytest.mark.parametrize("n,V,K,dtype,T", [
+    (9, 50, 40, torch.float32, 1.0), (5, 700, 6, torch.bfloat16, 1.0), (7, 4099, 64, torch.float32, 0.5),
+    (2, 131072, 300, torch.bfloat16, 1.0), (300, 16411, 40, torch.bfloat16, 1.0), (300, 8200, 128, torch.float32, 2.0),
+    (297, 80003, 33, torch.float32, 1.0)])
+def test_a_rest_far_below_the_ids(n, V, K, dtype, T, drop):
+    """Finite logits outside the teacher's ids, however far below the row's largest (peaked rows, small temperatures,
+    finite masks): the divergence is finite, and the gradient outside is -w T p_r softmax(outside).  Rows 0 and 1: one
+    entry outside is left, and none, where the divergence is infinite and the gradient outside zero.
+
+    Tolerances: exponents (z - m) / T and t / T - lse carry 2^-23 of their size, exponentials and sums 2^-17 in all (see
+    test_losses.py).  p_r is one minus a sum of p: delta absolutely, and log(p_r / q_r) multiplies it."""
+    import kdn_b200 as kdn
+
+    rng = np.random.default_rng(n + V + K)
+    ids = np.stack([rng.permutation(V)[:K] for _ in range(n)])
+    z = _logits(n, V, torch.float32, seed=V, scale=2.0)
+    top = torch.full((n, V), -drop * T, device="cuda")
+    idd, = _cuda(ids)
+    top.scatter_(1, idd, 3.0)
+    z = (z + top).to(dtype)
+    z.scatter_(1, idd, (torch.randn(n, K, device="cuda", generator=torch.Generator("cuda").manual_seed(1))).to(dtype))
+    one = (ids[0, 0] + 1) % V
+    while one in ids[0]:
+        one = (one + 1) % V
+    keep = torch.zeros(2, V, dtype=torch.bool, device="cuda").scatter_(1, idd[:2], True)
+    keep[0, one] = True
+    z[:2] = torch.where(keep, z[:2], -float("inf"))
+    t = np.sort(2.0 * rng.standard_normal((n, K)), axis=1)[:, ::-1].astype(np.float32).copy()
+    lse = (np.logaddexp.reduce(t.astype(np.float64) / T, axis=1) - np.log(0.6 + 0.3 * rng.random(n))).astype(np.float32)
+    w = ((0.5 + rng.random(n)) / n).astype(np.float32)
+    td, ld, wd = _cuda(t, lse, w)
+    loss, kl, d = kdn.distillation_loss_and_grad(z, td, idd, teacher_lse=ld, weights=wd, temperature=T)
+    plain = kdn.distillation_loss(z, td, idd, teacher_lse=ld, weights=wd, temperature=T)
+    assert torch.equal(plain[0], loss) and torch.equal(plain[1], kl) and float(loss) == float("inf")
+    got, g = _np(kl), _np(d)
+    assert got[1] == np.inf and np.isfinite(g[1]).all()
+    outside = np.ones(V, bool)
+    outside[ids[1]] = False
+    assert (g[1][outside] == 0).all()
+    delta = 2.0 ** -23 * (np.abs(t).max() / T + 20) + 2.0 ** -17
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    rows = range(n) if n < 50 else [0, *range(2, n, 13), n - 1]
+    for r in rows:
+        if r == 1:
+            continue
+        zr = _np(z[r])
+        want, p, q, p_r, log_qr, out, rel = _rest_reference(zr, T, t[r].astype(np.float64), ids[r], float(lse[r]))
+        X = 2.0 ** -23 * (zr.max() - zr[np.isfinite(zr)].min()) / T + 2.0 ** -17
+        assert abs(got[r] - want) <= 2 * X + delta * (abs(np.log(p_r) - log_qr) + 2)
+        c, total = float(w[r]) * T, p.sum() + p_r
+        ref = c * (total * np.exp(rel[out] + log_qr) - p_r * np.exp(rel[out]))
+        part = c * (total * np.exp(rel[out] + log_qr) + p_r * np.exp(rel[out]))
+        fin = rel[out][np.isfinite(rel[out])]
+        share = 4 * (2.0 ** -23 * (fin.max() - fin.min()) + 2.0 ** -17 + delta / p_r)
+        assert (np.abs(g[r][out] - ref) <= part * share + np.abs(ref) * half + 1e-37).all()
+        ref = c * (q * total - p)
+        assert (np.abs(g[r][ids[r]] - ref) <= 4 * c * (q + p) * (X + delta) + np.abs(ref) * half + 1e-37).all()
+
+
+@gpu
+@pytest.mark.parametrize("n,V,dtype", [(5, 700, torch.float32), (3, 131072, torch.bfloat16), (300, 16411, torch.bfloat16)])
+def test_a_teacher_without_a_rest_and_a_student_with_a_mask(n, V, dtype):
+    """All of the teacher's mass lies in its entries (one minus its sum is rounding alone) and the student's other logits
+    are masked, by -inf or by the type's lowest value: the divergence is that over the entries."""
+    import kdn_b200 as kdn
+
+    K = 40
+    rng = np.random.default_rng(V)
+    ids = np.stack([rng.permutation(V)[:K] for _ in range(n)])
+    idd, = _cuda(ids)
+    for mask in (-float("inf"), torch.finfo(dtype).min, -1e30):
+        z = torch.full((n, V), mask, device="cuda").to(dtype)
+        z.scatter_(1, idd, _logits(n, K, dtype, seed=5, scale=2.0))
+        t = (2.0 * rng.standard_normal((n, K))).astype(np.float32)
+        lse = np.logaddexp.reduce(t.astype(np.float64), axis=1).astype(np.float32)
+        td, ld = _cuda(t, lse)
+        loss, kl, d = kdn.distillation_loss_and_grad(z, td, idd, teacher_lse=ld)
+        want = oracle.distillation_loss(np.take_along_axis(_np(z), ids, 1), t, np.tile(np.arange(K), (n, 1)))
+        assert np.abs(_np(kl) - want[1]).max() <= 2.0 ** -16
+        # p_r, at most 2^-20, is left out
+        g = np.take_along_axis(_np(d), ids, 1)
+        half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+        assert (np.abs(g - want[2]) <= 2.0 ** -16 / n + half * np.abs(want[2])).all()
+        assert torch.equal(d.scatter(1, idd, 0.0), torch.zeros_like(d))
