@@ -355,7 +355,8 @@ int kdn_varlen_causal_attention(const void* q, const void* k_cache, const void* 
  * to -inf have probability zero; a row of nothing else, or with a NaN or +inf, gives NaN.
  *
  * A row whose label is ignore_index counts for nothing: its logits are not read, its outputs and its gradient row are
- * zero.  A label outside [0, V) is treated the same way and recorded for kdn_device_error (code 1).  weights [n] fp32
+ * zero.  A label outside [0, V) is treated the same way and recorded for kdn_device_error (code 1): neither is part of
+ * a mean over the rows that count or of a sequence's number of rows.  weights [n] fp32
  * multiply each row's loss (a row of weight zero adds nothing to the loss or the gradient, whatever it holds); NULL
  * means the mean over the rows that count.  Nothing here depends on an order of atomics: equal calls give equal bits.
  *
@@ -372,7 +373,7 @@ int kdn_varlen_causal_attention(const void* q, const void* k_cache, const void* 
  *     log sigmoid(-h).  A sequence of no counting row has log ratio 0.
  *   kdn_distillation_loss: the teacher's `top` largest logits of each row and their ids [n, top] (ids in index_dtype;
  *     negative ids are padding, and a row whose FIRST id is negative counts for nothing; an id >= V is skipped and
- *     recorded, code 1; an id given twice counts twice).  teacher_lse NULL: p = softmax of the row's entries / T; else
+ *     recorded, code 1, without a change to whether its row counts; an id given twice counts twice).  teacher_lse NULL: p = softmax of the row's entries / T; else
  *     p = e^(teacher / T - teacher_lse[t]) (log-sum-exp of the teacher's whole row / T) and what is left of the
  *     teacher's mass, 1 - sum p, is compared with the student's mass outside the ids as one more class, however far below
  *     the ids' its logits lie (where all of them are -inf the divergence is +inf and the gradient outside the ids zero;

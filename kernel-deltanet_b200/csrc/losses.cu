@@ -410,6 +410,11 @@ __device__ __forceinline__ S merge_rows(S a, const LossRows& r, int rank, int pa
   return a;
 }
 
+// a row counts when its label is not ignore_index and lies in the vocabulary
+__device__ __forceinline__ bool counts(int64_t y, int64_t ignore_index, int64_t V) {
+  return y != ignore_index && y >= 0 && y < V;
+}
+
 // the label of a row, or -1 for a row that counts for nothing (its label is ignore_index; a label outside
 // the vocabulary is recorded and treated the same way)
 __device__ __forceinline__ int64_t row_label(const LossRows& a, int64_t r, bool record) {
@@ -459,13 +464,14 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, const Poli
   return p;
 }
 
-// 1 / (rows that count) for a few rows, by every warp that asks: rows whose label is not ignore_index, or (ids) whose
-// first id is not negative.
+// 1 / (rows that count) for a few rows, by every warp that asks: by their labels, or (ids) those whose first id is not
+// negative.
 constexpr int64_t kFewRows = 256;
 __device__ __forceinline__ float mean_of_few(const LossRows& a, const void* ids, int K) {
   int live = 0;
   for (int64_t r = threadIdx.x & 31; r < a.n; r += 32)
-    live += ids ? ld_index(ids, a.index_dtype, r * K) >= 0 : ld_index(a.labels, a.index_dtype, r) != a.ignore_index;
+    live += ids ? ld_index(ids, a.index_dtype, r * K) >= 0
+                : counts(ld_index(a.labels, a.index_dtype, r), a.ignore_index, a.V);
   live = __reduce_add_sync(0xffffffffu, live);
   return live > 0 ? 1.f / float(live) : 0.f;
 }
@@ -1649,16 +1655,16 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
 }
 
 // The two sums over rows, one CTA each (a fixed order): latency, 2 to 3 us after the kernel before them.
-// scale = 1 / (rows that count): rows whose label is not ignore_index, or (K > 0) whose first id is >= 0
+// scale = 1 / (rows that count): by their labels, or (by_sign) those whose first id is not negative
 __global__ void __launch_bounds__(1024) live_scale_kernel(const void* __restrict__ labels, int index_dtype, int64_t n,
-                                                          int64_t stride, bool by_sign, int64_t ignore_index,
+                                                          int64_t stride, bool by_sign, int64_t ignore_index, int64_t V,
                                                           float* __restrict__ scale) {
   await_previous();
   __shared__ double red[32];
   int64_t c = 0;
   for (int64_t r = threadIdx.x; r < n; r += 1024) {
     const int64_t y = ld_index(labels, index_dtype, r * stride);
-    c += by_sign ? y >= 0 : y != ignore_index;
+    c += by_sign ? y >= 0 : counts(y, ignore_index, V);
   }
   const double live = block_sum_f64(double(c), red);
   if (threadIdx.x == 0) *scale = live > 0.0 ? float(1.0 / live) : 0.f;
@@ -1700,9 +1706,8 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(LossRows a, PairTerm
   const auto token = [&](int64_t r) {
     Token k{0.0, 0.0, false};
     const int64_t y = ld_index(a.labels, a.index_dtype, r);
-    if (y == a.ignore_index) return k;
+    if (!counts(y, a.ignore_index, a.V)) return k;  // (one outside the vocabulary is recorded by the forward kernel)
     ++count;
-    if (y < 0 || y >= a.V) return k;  // recorded by the forward kernel
     k.use = true;
     k.z = double(ld_as_f32(a.logits, a.dtype, r * a.ld + y));
     k.ref = t.ref ? double(t.ref[r]) : 0.0;
@@ -1985,7 +1990,7 @@ cudaError_t launch_policy_loss(const LossRows& a, PolicyTerms t, float* loss, cu
   const bool mean = t.scale != nullptr;
   if (mean) {
     const cudaError_t e = launch(live_scale_kernel, 1, 1024, 1, 0, false, stream, a.labels, a.index_dtype, a.n, 1,
-                                 false, a.ignore_index, const_cast<float*>(t.scale));
+                                 false, a.ignore_index, a.V, const_cast<float*>(t.scale));
     if (e != cudaSuccess) return e;
   }
   if (cudaError_t e = launch_logp(a, t, mean, stream); e != cudaSuccess) return e;
@@ -2010,7 +2015,7 @@ cudaError_t launch_distillation_loss(const LossRows& a, DistillTerms t, float* l
   const bool mean = t.scale != nullptr;
   if (mean) {
     const cudaError_t e = launch(live_scale_kernel, 1, 1024, 1, 0, false, stream, t.ids, a.index_dtype, a.n, t.K, true,
-                                 0, const_cast<float*>(t.scale));
+                                 0, a.V, const_cast<float*>(t.scale));
     if (e != cudaSuccess) return e;
   }
   if (cudaError_t e = launch_distill(a, t, mean, stream); e != cudaSuccess) return e;

@@ -223,3 +223,35 @@ def test_a_teacher_without_a_rest_and_a_student_with_a_mask(n, V, dtype):
         half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
         assert (np.abs(g - want[2]) <= 2.0 ** -16 / n + half * np.abs(want[2])).all()
         assert torch.equal(d.scatter(1, idd, 0.0), torch.zeros_like(d))
+
+
+# ------------------------------------------------------------------------------------ labels outside the vocabulary
+@gpu
+@pytest.mark.parametrize("n,V", [(9, 300), (700, 300), (300, 16411)])
+@pytest.mark.parametrize("index", [torch.int64, torch.int32])
+def test_labels_outside_the_vocabulary_count_as_ignored_ones(n, V, index):
+    """In the mean over the rows that count and in a sequence's length, too: equal bits."""
+    import kdn_b200 as kdn
+
+    rng = np.random.default_rng(n)
+    z = _logits(n, V, torch.bfloat16, seed=1)
+    wrong, right = (torch.from_numpy(rng.integers(0, V, n)).cuda().to(index) for _ in range(2))
+    wrong[1::4], wrong[2::4], wrong[3::8] = V, -7, -100
+    right = torch.where((wrong < 0) | (wrong >= V), -100, wrong)
+    old = kdn.token_logprobs(z, right) - 0.1
+    adv = torch.ones_like(old)
+    assert _device_error() == 0
+    for call in (lambda y: kdn.policy_loss_and_grad(z, y, old, adv),
+                 lambda y: kdn.policy_loss(z, y, old, adv),
+                 lambda y: kdn.preference_loss_and_grad(z, y, torch.tensor([0, n // 3, n], device="cuda"), old + 0.3,
+                                                        beta=0.5, length_normalised=True)):
+        want = call(right)
+        assert _device_error() == 0
+        got = call(wrong)
+        assert _device_error() == 1
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    some = int((right >= 0).sum())
+    loss, _, _, d = kdn.policy_loss_and_grad(z, wrong, old, adv, clip_high=1e9)
+    assert _device_error() == 1
+    assert abs(float(loss) + np.exp(0.1)) < 1e-4  # every ratio is e^0.1: so is their mean, over `some` of n rows
+    assert 0 < some < n
