@@ -24,6 +24,7 @@
 
 #include "kdn_common.cuh"
 #include "kdn_internal.h"
+#include "loss_plan.h"
 #include "tc_prims.cuh"
 
 namespace kdn {
@@ -33,8 +34,6 @@ __device__ int g_loss_error;
 namespace {
 
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kMaxCluster = 8;
-constexpr int kNV = 8;  // vectors of a share that a thread keeps in registers
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -439,9 +438,11 @@ struct PolicyRow {
 struct PolicyIn {
   float w, adv, old, ref;
 };
+// (kCounted: the weight stands in memory; else, without weights and scale, the caller counts the rows)
+template <bool kCounted>
 __device__ __forceinline__ PolicyIn policy_inputs(const PolicyTerms& t, int64_t r) {
-  if (!t.row_loss) return PolicyIn{};
-  return PolicyIn{t.weights ? t.weights[r] : t.scale ? *t.scale : 0.f, t.advantages[r], t.old_logps[r],
+  if (!kCounted && !t.row_loss) return PolicyIn{};
+  return PolicyIn{t.weights ? t.weights[r] : kCounted || t.scale ? *t.scale : 0.f, t.advantages[r], t.old_logps[r],
                   t.ref_logps ? t.ref_logps[r] : 0.f};
 }
 __device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, const PolicyIn& in, float logp, float H) {
@@ -466,7 +467,6 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyTerms& t, const Poli
 
 // 1 / (rows that count) for a few rows, by every warp that asks: by their labels, or (ids) those whose first id is not
 // negative.
-constexpr int64_t kFewRows = 256;
 __device__ __forceinline__ float mean_of_few(const LossRows& a, const void* ids, int K) {
   int live = 0;
   for (int64_t r = threadIdx.x & 31; r < a.n; r += 32)
@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
   }
   if (parts > 1) tc::cluster_arrive();
   const float zy = to_f32(w.z[y]);
-  PolicyIn in = policy_inputs(t, r);
+  PolicyIn in = policy_inputs<false>(t, r);
   uint4 v[kNV];
   auto load = [&](int at) {
 #pragma unroll
@@ -824,18 +824,15 @@ __global__ void __launch_bounds__(Cta<NT>::kThreads, 1024 / Cta<NT>::kThreads)
 // stays in the ring until its gradient is written, and the ring holds three of 64 KB, so the time from a row's last
 // chunk to its coefficients counts in full.  Other shapes of the ring and the roles, the same policy loss: 256 threads
 // x 4 vectors 748 us (kept); x 3 828, x 2 867, x 5 810, x 6 817; 320 threads x 3 813, 384 x 3 833, 384 x 2 815.
-constexpr int kPer = 4;                // vectors that a thread of a role takes at a time
 constexpr int kBuf = 8;                // rows between a partial result and its use, see Exchange
 constexpr int kQueue = 32;             // rows between the producer and the last of the other roles
-constexpr int kRoleThreads = 256;      // of the statistics and of the gradient role
 constexpr int kRoleWarps = kRoleThreads / 32;
 constexpr int kControlWarps = 2;
 constexpr int kMaxTop = 128;           // teacher entries of a row that the streaming kernel takes
 constexpr int kTeachers = 6;           // rows between the teacher and the patcher (even: control takes rows in turn)
 constexpr uint32_t kLossWaitLimit = 1u << 20;
-constexpr int kChunk = kPer * kRoleThreads;  // vectors: 16 KiB
 
-constexpr int kSlots = 13;                   // chunks of the ring
+constexpr int kSlots = 13;             // chunks of the ring
 constexpr size_t kRingBytes = size_t(kSlots) * kChunk * 16;
 
 // What the kinds of losses differ in: their roles.
@@ -1234,7 +1231,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
         if constexpr (!kDistill) {
           // asked for while the row's statistics are still being formed
           const float zy = to_f32((logits + row.row * a.ld)[row.label]);
-          const PolicyIn in = policy_inputs(t, row.row);
+          const PolicyIn in = policy_inputs<true>(t, row.row);
           ok = wait_cluster(&x.part_full[buf.i], buf.parity);
           if (!ok) break;
           const auto st = merge_parts<Stats<true>>(x.part + buf.i * row_parts, row_parts, a);
@@ -1803,39 +1800,13 @@ __global__ void __launch_bounds__(kSmall) scale_kernel(LossRows a, const float* 
 }
 
 // ------------------------------------------------------------------------------------------------- launches
-// How a row is split: threads of a CTA and CTAs of a row's cluster.
-struct Split {
-  int threads, parts;  // threads of a row's CTA (32: a warp of one with four rows), CTAs of a row's cluster
-};
-
 // the most 16-byte vectors that a row reaches into
 int64_t row_vectors(const LossRows& a) {
   const int64_t E = a.dtype == KDN_DTYPE_BF16 ? 8 : 4;
   const bool aligned = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && (a.ld % E == 0 || a.n == 1);
   return aligned ? (a.V + E - 1) / E : (a.V + 2 * E - 2) / E;
 }
-
-// Kernels that keep a row's share in registers.  Many short rows: a warp each (B200, policy loss with gradient, bf16,
-// 16384 x 1000: 27 us against 74 with 128 threads a row; 16384 x 4096: 65 against 92, but 600 x 4096: 10.8 against
-// 9.1).  Else enough threads to hold the row, over more CTAs where one is too small, but (few rows being spread over
-// the SMs at best) no more than two CTAs an SM.
-Split choose_split(const LossRows& a) {
-  const int64_t vecs = row_vectors(a), sms = current_sm_count();
-  if ((vecs <= 256 && a.n >= 2 * sms) || (vecs <= 512 && a.n >= 8 * sms)) return Split{32, 1};
-  Split s{vecs <= 128 * kNV ? 128 : vecs <= 256 * kNV ? 256 : 512, 1};
-  while (s.parts < kMaxCluster && vecs > int64_t(s.threads) * kNV * s.parts && a.n * s.parts < 2 * sms) s.parts *= 2;
-  return s;
-}
-
-// Log-probabilities alone read a row once and keep nothing of it: where there are rows enough, small CTAs in as many
-// rounds as it takes (at different places of their rows, those of an SM keep the memory busy).  B200, bf16:
-// 16384 x 4096 26 us with a warp a row, 53 with 128 threads; 4096 x 32000 47 us with 128 threads, 65 with the row in
-// the registers of 512; 2400 x 131072 101 us with 256 threads, 107 with 128, 326 with a cluster of four times 512.
-Split choose_scan_split(const LossRows& a) {
-  if (a.n < 2 * current_sm_count()) return choose_split(a);
-  const int64_t vecs = row_vectors(a);
-  return Split{vecs <= 1024 ? 32 : vecs <= 8192 ? 128 : 256, 1};
-}
+LossShape shape_of(const LossRows& a) { return {a.n, row_vectors(a), current_sm_count()}; }
 
 // One launch.  `after`: the previous one on the stream is of the same call, and this one's start may overlap its end.
 template <typename... KArgs, typename... Args>
@@ -1885,45 +1856,18 @@ cudaError_t dispatch(const LossRows& a, Split s, F f) {
   return f(float{}, integral_constant<int, 512>{});
 }
 
-// The CTAs of a row's cluster and the vectors of each one's share in the streaming kernel; parts = 0: the rows are too
-// long for its ring, which has to hold a row's share and what is being copied of the next one's, or it does not pay:
-// rows of up to 32 KiB, or fewer than two an SM.  Measured on B200, policy loss with gradient, bf16, streaming kernel
-// against CTAs that keep a row in registers: 2400 x 4096 30.3 us against 18.8, 148 x 32000 11.5 against 9.4, 600 x
-// 32000 26.8 against 26.1, 2400 x 32000 69.4 against 77.2, 2400 x 131072 236 against 330.  The choice does not depend
-// on whether a gradient is asked for, so that the outputs do not either.
-struct Stream {
-  int parts, per;
-};
-Stream choose_stream(const LossRows& a) {
-  const int64_t vecs = row_vectors(a);
-  if (vecs <= 2048 || a.n < 2 * current_sm_count()) return {0, 0};
-  for (int parts = 1; parts <= kMaxCluster; parts *= 2) {
-    const int64_t per = (vecs + parts - 1) / parts;
-    if (per <= 9 * kChunk) return {parts, int(per)};
-  }
-  return {0, 0};
-}
-
-// Rows of one request: as many as make 128 KiB, as long as that leaves every SM sixteen requests to even out what
-// ignored rows save.
-int64_t group_rows(const LossRows& a, Stream s) {
-  const int64_t chunks = (s.per + kChunk - 1) / kChunk, most = a.n * s.parts / (16 * current_sm_count());
-  return std::max<int64_t>(1, std::min<int64_t>(8 / chunks, most));
-}
-
 template <typename Terms, typename K>
 cudaError_t launch_stream(K kernel, const LossRows& a, const Terms& t, Stream s, bool after, cudaStream_t stream) {
   using S = Streaming<Terms>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRingBytes));
       e != cudaSuccess)
     return e;
-  const int64_t group = group_rows(a, s);
+  const int64_t group = group_rows(shape_of(a), s);
   return launch_rows(kernel, (a.n + group - 1) / group, Split{S::kThreads, s.parts}, true, kRingBytes, after,
                      stream, a, t, int(group), s.per);
 }
 
-cudaError_t launch_logp(const LossRows& a, const PolicyTerms& t, bool after, cudaStream_t stream) {
-  const Stream st = t.row_loss ? choose_stream(a) : Stream{0, 0};
+cudaError_t launch_logp(const LossRows& a, const PolicyTerms& t, Stream st, bool after, cudaStream_t stream) {
   if (st.parts > 0) {
     const auto go = [&](auto z) {
       using T = decltype(z);
@@ -1933,7 +1877,7 @@ cudaError_t launch_logp(const LossRows& a, const PolicyTerms& t, bool after, cud
     };
     return a.dtype == KDN_DTYPE_BF16 ? go(__nv_bfloat16{}) : go(float{});
   }
-  const Split s = t.row_loss ? choose_split(a) : choose_scan_split(a);
+  const Split s = t.row_loss ? choose_split(shape_of(a)) : choose_scan_split(shape_of(a));
   return dispatch(a, s, [&](auto z, auto nt) {
     using T = decltype(z);
     constexpr int NT = decltype(nt)::value;
@@ -1944,8 +1888,7 @@ cudaError_t launch_logp(const LossRows& a, const PolicyTerms& t, bool after, cud
   });
 }
 
-cudaError_t launch_distill(const LossRows& a, const DistillTerms& t, bool after, cudaStream_t stream) {
-  const Stream st = t.K <= kMaxTop ? choose_stream(a) : Stream{0, 0};
+cudaError_t launch_distill(const LossRows& a, const DistillTerms& t, Stream st, bool after, cudaStream_t stream) {
   if (st.parts > 0) {
     const auto go = [&](auto z) {
       using T = decltype(z);
@@ -1954,7 +1897,7 @@ cudaError_t launch_distill(const LossRows& a, const DistillTerms& t, bool after,
     };
     return a.dtype == KDN_DTYPE_BF16 ? go(__nv_bfloat16{}) : go(float{});
   }
-  Split s = choose_split(a);
+  Split s = choose_split(shape_of(a));
   s.threads = std::max(s.threads, 128);
   return dispatch(a, s, [&](auto z, auto nt) {
     using T = decltype(z);
@@ -1970,7 +1913,7 @@ cudaError_t launch_distill(const LossRows& a, const DistillTerms& t, bool after,
 }  // namespace
 
 cudaError_t launch_token_logprobs(const LossRows& a, cudaStream_t stream) {
-  return launch_logp(a, PolicyTerms{}, false, stream);
+  return launch_logp(a, PolicyTerms{}, Stream{0, 0}, false, stream);
 }
 
 cudaError_t launch_token_logprobs_backward(const LossRows& a, const float* dlogps, bool after, cudaStream_t stream) {
@@ -1986,14 +1929,15 @@ cudaError_t launch_token_logprobs_backward(const LossRows& a, const float* dlogp
 }
 
 cudaError_t launch_policy_loss(const LossRows& a, PolicyTerms t, float* loss, cudaStream_t stream) {
-  if (t.weights || a.n <= kFewRows) t.scale = nullptr;  // few rows: their own kernel counts
-  const bool mean = t.scale != nullptr;
+  const Stream st = choose_stream(shape_of(a));
+  const bool mean = !t.weights && !counts_rows_itself(shape_of(a), st);
+  if (!mean) t.scale = nullptr;
   if (mean) {
     const cudaError_t e = launch(live_scale_kernel, 1, 1024, 1, 0, false, stream, a.labels, a.index_dtype, a.n, 1,
                                  false, a.ignore_index, a.V, const_cast<float*>(t.scale));
     if (e != cudaSuccess) return e;
   }
-  if (cudaError_t e = launch_logp(a, t, mean, stream); e != cudaSuccess) return e;
+  if (cudaError_t e = launch_logp(a, t, st, mean, stream); e != cudaSuccess) return e;
   return launch(loss_sum_kernel, 1, 1024, 1, 0, true, stream, t.row_loss, a.n, 1.0, loss);
 }
 
@@ -2002,7 +1946,7 @@ cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, cudaSt
   f.dlogits = nullptr;
   f.coef_zero = t.coef;
   f.pairs_done = t.pairs_done;
-  cudaError_t e = a.n > 0 ? launch_logp(f, PolicyTerms{}, false, stream)
+  cudaError_t e = a.n > 0 ? launch_logp(f, PolicyTerms{}, Stream{0, 0}, false, stream)
                           : cudaMemsetAsync(t.pairs_done, 0, sizeof(unsigned), stream);
   if (e != cudaSuccess) return e;
   e = launch(pair_kernel, t.pairs, kPairThreads, 1, 0, a.n > 0, stream, a, t);
@@ -2011,14 +1955,15 @@ cudaError_t launch_preference_loss(const LossRows& a, const PairTerms& t, cudaSt
 }
 
 cudaError_t launch_distillation_loss(const LossRows& a, DistillTerms t, float* loss, cudaStream_t stream) {
-  if (t.weights || a.n <= kFewRows) t.scale = nullptr;  // few rows: their own kernel counts
-  const bool mean = t.scale != nullptr;
+  const Stream st = t.K <= kMaxTop ? choose_stream(shape_of(a)) : Stream{0, 0};
+  const bool mean = !t.weights && !counts_rows_itself(shape_of(a), st);
+  if (!mean) t.scale = nullptr;
   if (mean) {
     const cudaError_t e = launch(live_scale_kernel, 1, 1024, 1, 0, false, stream, t.ids, a.index_dtype, a.n, t.K, true,
                                  0, a.V, const_cast<float*>(t.scale));
     if (e != cudaSuccess) return e;
   }
-  if (cudaError_t e = launch_distill(a, t, mean, stream); e != cudaSuccess) return e;
+  if (cudaError_t e = launch_distill(a, t, st, mean, stream); e != cudaSuccess) return e;
   return launch(loss_sum_kernel, 1, 1024, 1, 0, true, stream, t.row_loss, a.n, 1.0, loss);
 }
 
