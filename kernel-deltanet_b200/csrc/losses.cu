@@ -550,6 +550,13 @@ __device__ __forceinline__ float mass_at(const int* ids, const float* lp, int K,
   return p;
 }
 
+// the first entry of the same id as entry k
+__device__ __noinline__ int first_of(const int* ids, int k) {
+  int i = 0;
+  while (ids[i] != ids[k]) ++i;
+  return i;
+}
+
 // The row's softmax from the student's sums outside the ids and at them, and what is left of the teacher: p_r = 1 - P,
 // P = sum p, where the rest is a class of its own (else zero).  Where the student has nothing left, or less than an fp32
 // number of the row's own scale could hold (q_r < 2^-126), a p_r of the size of P's rounding is none: times log q_r it
@@ -1408,7 +1415,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
             any |= here[i];
           }
           if (__any_sync(0xffffffffu, any)) {
-            // every entry leaves its number; the one that is found there counts, the others are the same id again
+            // every entry leaves its number; where another one's is found there, the same id was given again
             uint32_t bits[kMaxTop / 32], found[kMaxTop / 32];
 #pragma unroll
             for (int i = 0; i < kMaxTop / 32; ++i) bits[i] = get_bits<T>(place[i]);
@@ -1423,12 +1430,19 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
             for (int i = 0; i < kMaxTop / 32; ++i) put_bits<T>(place[i], Vec<T>::kFill);
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&x.marked[slot.i]);
+            uint32_t differ = 0u;
+#pragma unroll
+            for (int i = 0; i < kMaxTop / 32; ++i) differ |= here[i] ? found[i] ^ uint32_t(lane + 32 * i) : 0u;
+            if (__any_sync(0xffffffffu, differ)) {  // the first entry of an id counts, whichever store came last
+              again = true;
+#pragma unroll
+              for (int i = 0; i < kMaxTop / 32; ++i)
+                if (here[i]) here[i] = first_of(x.teacher[teach.i].id, lane + 32 * i) == lane + 32 * i;
+            }
             float m = st.m;
 #pragma unroll
             for (int i = 0; i < kMaxTop / 32; ++i) {
-              const bool own = found[i] == uint32_t(lane + 32 * i);
-              again |= here[i] && !own;
-              here[i] = here[i] && own && bits_to_f32<T>(bits[i]) != -INFINITY;
+              here[i] = here[i] && bits_to_f32<T>(bits[i]) != -INFINITY;
               if (here[i]) m = fmaxf(m, bits_to_f32<T>(bits[i]));
             }
             rescale(st, m, a);
@@ -1439,7 +1453,6 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
             tc::mbar_arrive(&x.marked[slot.i]);
           }
         }
-        again = __any_sync(0xffffffffu, again);
         if (lane == 0 && kGrad != 0) {
           x.twice[teach.i] = again;
           tc::mbar_arrive(&x.row_done[teach.i]);
@@ -1571,16 +1584,19 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
       const int vi = (id[k] + w.off) / Vec<T>::E - at;
       if (vi < 0 || vi >= NT * kNV || vi + at >= w.v1) continue;
       const uint32_t bit = 1u << (8 * (vi & 3) + (id[k] + w.off) % Vec<T>::E);
-      if (atomicOr(&mark[vi >> 2], bit) & bit) {
-        twice = 1;
-      } else if (kTail) {
+      if (atomicOr(&mark[vi >> 2], bit) & bit) twice = 1;
+    }
+    __syncthreads();
+    if constexpr (kTail) {
+      for (int k = tid; k < K; k += NT) {
+        const int vi = (id[k] + w.off) / Vec<T>::E - at;
+        if (id[k] < 0 || vi < 0 || vi >= NT * kNV || vi + at >= w.v1) continue;
+        if (twice && first_of(id, k) != k) continue;  // by its place, not by which thread came first
         const float zk = to_f32(w.z[id[k]]), m = fmaxf(st.in.m, zk);
         rescale(st.in, m, a);
         st.in.s += zk == -INFINITY ? 0.f : ex2((zk - m) * a.k);
       }
-    }
-    __syncthreads();
-    if constexpr (kTail) {  // (their entries of the gradient are written over in any case)
+      // the vectors without the ids' logits (their entries of the gradient are written over in any case)
 #pragma unroll
       for (int i = 0; i < kNV; ++i) {
         const uint32_t bits = reinterpret_cast<const uint8_t*>(mark)[tid + i * NT];

@@ -255,3 +255,26 @@ def test_labels_outside_the_vocabulary_count_as_ignored_ones(n, V, index):
     assert _device_error() == 1
     assert abs(float(loss) + np.exp(0.1)) < 1e-4  # every ratio is e^0.1: so is their mean, over `some` of n rows
     assert 0 < some < n
+
+
+# ------------------------------------------------------------------------------------------------- ids given twice
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,K", [(64, 4100, 128), (64, 4100, 200), (3, 131072, 1024), (300, 16411, 128)])
+def test_an_id_given_twice_gives_equal_bits(n, V, K, dtype):
+    """Whatever warps its entries belong to: 3 and 100, 7 and 40, 9 and the last."""
+    import kdn_b200 as kdn
+
+    rng = np.random.default_rng(K)
+    z = _logits(n, V, dtype, seed=3)
+    ids = np.stack([rng.permutation(V)[:K] for _ in range(n)])
+    ids[:, 100], ids[:, 40], ids[:, -1] = ids[:, 3], ids[:, 7], ids[:, 9]
+    t = (2.0 * rng.standard_normal((n, K))).astype(np.float32)
+    lse = (np.logaddexp.reduce(t.astype(np.float64), axis=1) + 0.2).astype(np.float32)
+    td, idd, ld = _cuda(t, ids, lse)
+    want = kdn.distillation_loss_and_grad(z, td, idd, teacher_lse=ld)
+    ref = oracle.distillation_loss(_np(z), t, ids, lse)
+    assert np.abs(_np(want[1]) - ref[1]).max() <= 30 * (2.0 ** -17 + 2.0 ** -23 * 60)
+    for _ in range(100):
+        got = kdn.distillation_loss_and_grad(z, td, idd, teacher_lse=ld)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
