@@ -1337,6 +1337,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
           if (kDistill) tc::fence_proxy_async_smem();  // the marker has written to the slot: the copy comes after
           const uint32_t dst = ring + uint32_t(slot.i * kChunk) * 16u;
           int lo = at, hi = min(at + kChunk, sh.count);
+          const int count = hi - lo;
           if (head && lo == 0) {
             sts16(dst, load_edge(z, -sh.off, V));
             ++lo;
@@ -1345,6 +1346,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
             --hi;
             sts16(dst + (hi - at) * 16, load_edge(z, (sh.v0 + hi) * E - sh.off, V));
           }
+          if (hi - lo < count) tc::fence_proxy_async_smem();  // these stores before the slot's next copy
           const uint32_t bytes = uint32_t(hi - lo) * 16u;
           if (bytes) {
             tc::mbar_arrive_expect_tx(&x.full[slot.i], bytes);
