@@ -1290,7 +1290,8 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
     // Group k's rows are copied while the answer about group k + 2 is on its way: group k + 1's is read, and passed on
     // to the cluster, before group k is begun.
     int group = int(blockIdx.x) / parts, next = -1;
-    if (rank == 0 && lane == 0) request_rows(&x.response, &x.response_full);
+    bool asked = rank == 0;  // an answer is on its way
+    if (asked && lane == 0) request_rows(&x.response, &x.response_full);
     while (ok && group >= 0) {
       const int64_t first = int64_t(group) * group_rows;
       const int rows = int(min(int64_t(group_rows), a.n - first));
@@ -1305,13 +1306,16 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
       }
       if (rank == 0) {
         const bool answered = warp_wait(&x.response_full, response_parity);
-        response_parity ^= 1u;
         const int64_t cta = answered ? requested_cta(&x.response) : -1;
         next = __shfl_sync(0xffffffffu, cta < 0 ? -1 : int(cta / parts), 0);
         ok = ok && answered;
-        tc::fence_proxy_async_smem();  // read before the next answer is written there
-        __syncwarp();
-        if (next >= 0 && lane == 0) request_rows(&x.response, &x.response_full);
+        if (answered) {
+          asked = next >= 0;
+          response_parity ^= 1u;
+          tc::fence_proxy_async_smem();  // read before the next answer is written there
+          __syncwarp();
+          if (asked && lane == 0) request_rows(&x.response, &x.response_full);
+        }
         if (parts > 1) {
           if (tk.wrapped) ok = wait_cluster(&x.ticket_free[tk.i], tk.parity ^ 1u) && ok;
           if (lane < parts) {
@@ -1364,7 +1368,7 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
       }
       group = next;
     }
-    if (!ok && rank == 0 && next >= 0)  // an answer is on its way: it lands before the CTA leaves
+    if (!ok && asked)  // the answer lands before the CTA leaves
       tc::mbar_wait_bounded(&x.response_full, response_parity, 1u << 16);
     push(-1, -1);
     if (!ok)  // copies in flight land before the CTA leaves: wait for every slot's last use
