@@ -14,11 +14,11 @@ q = softmax(x):
 
 Logits are float32 or bfloat16, [..., vocab], with any row stride and alignment; the formulas, what ignored rows,
 weights and padding mean, and what -inf and NaN give stand at the entries of include/kdn.h.  Only logits receive a
-gradient.  The loss and its gradient come from one pass over the logits (two for ``preference_loss``), so
-``loss.backward()`` only hands over what the forward formed (scaled by the upstream gradient where that is not
-one); the logits are not kept.  A second backward through one call raises.  ``*_loss_and_grad`` return the
-gradient directly, as a last value, for trainers that run their own head backward.  Losses, log-probabilities and
-statistics are float32.  Errors raise RuntimeError; there is no CPU path.
+gradient, and in reverse mode alone: logits with a forward-mode tangent are refused.  The loss and its gradient come
+from one pass over the logits (two for ``preference_loss``), so ``loss.backward()`` only hands over what the forward
+formed (scaled by the upstream gradient where that is not one); the logits are not kept.  A second backward through one
+call raises.  ``*_loss_and_grad`` return the gradient directly, as a last value, for trainers that run their own head
+backward.  Losses, log-probabilities and statistics are float32.  Errors raise RuntimeError; there is no CPU path.
 """
 
 from __future__ import annotations
@@ -26,6 +26,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as fwad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -59,6 +60,8 @@ def _rows(logits: torch.Tensor) -> torch.Tensor:
         raise RuntimeError(f"logits must be float32 or bfloat16, got {logits.dtype}")
     if logits.dim() < 2 or logits.shape[-1] < 1:
         raise RuntimeError(f"logits must be [..., vocab], got {tuple(logits.shape)}")
+    if fwad.unpack_dual(logits).tangent is not None:
+        raise RuntimeError("the losses over logits have no forward-mode derivative")
     z = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     if z.stride(1) != 1 and z.shape[1] > 1 or z.shape[0] > 1 and z.stride(0) < z.shape[1]:
         z = z.contiguous()

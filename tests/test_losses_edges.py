@@ -278,3 +278,27 @@ def test_an_id_given_twice_gives_equal_bits(n, V, K, dtype):
     for _ in range(100):
         got = kdn.distillation_loss_and_grad(z, td, idd, teacher_lse=ld)
         assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+# ------------------------------------------------------------------------------------------------- autograd's surface
+@gpu
+def test_forward_mode_is_refused():
+    """A tangent of the logits is not dropped."""
+    import torch.autograd.forward_ad as fwad
+
+    import kdn_b200 as kdn
+
+    z, y, f = _logits(4, 33, torch.float32), torch.arange(4, device="cuda"), torch.zeros(4, device="cuda")
+    cu, ids = torch.tensor([0, 2, 4], device="cuda"), torch.arange(8, device="cuda").view(4, 2)
+    st = torch.ones(4, 2, device="cuda")
+    calls = [lambda x: kdn.token_logprobs(x, y), lambda x: kdn.token_logprobs_backward(x, y, st, f),
+             lambda x: kdn.policy_loss(x, y, f, f), lambda x: kdn.policy_loss_and_grad(x, y, f, f),
+             lambda x: kdn.preference_loss(x, y, cu), lambda x: kdn.preference_loss_and_grad(x, y, cu),
+             lambda x: kdn.distillation_loss(x, z[:, :2], ids), lambda x: kdn.distillation_loss_and_grad(x, z[:, :2], ids)]
+    for call in calls:
+        call(z)
+        with fwad.dual_level():
+            call(z)
+            for x in (z, z.detach().requires_grad_()):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(fwad.make_dual(x, torch.ones_like(z)))
