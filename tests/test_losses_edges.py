@@ -302,3 +302,30 @@ def test_forward_mode_is_refused():
             for x in (z, z.detach().requires_grad_()):
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     call(fwad.make_dual(x, torch.ones_like(z)))
+
+
+@gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_outputs_of_a_call_are_tensors_of_their_own(grad):
+    """Writing to one in place does not invalidate a graph that has kept another."""
+    import kdn_b200 as kdn
+
+    n = 6
+    z = _logits(n, 33, torch.float32).requires_grad_(grad)
+    y, f = torch.arange(n, device="cuda"), torch.zeros(n, device="cuda")
+    cu, ids = torch.tensor([0, 2, n], device="cuda"), torch.arange(2 * n, device="cuda").view(n, 2)
+    for call in (lambda: kdn.policy_loss(z, y, f, f), lambda: kdn.preference_loss(z, y, cu),
+                 lambda: kdn.distillation_loss(z, z.detach()[:, :2].contiguous(), ids),
+                 lambda: kdn.policy_loss_and_grad(z.detach(), y, f, f)):
+        count = len(call())
+        for kept in range(count):
+            for written in range(count):
+                if written == kept:
+                    continue
+                out = [o.detach() if o.requires_grad else o for o in call()]
+                w = torch.ones_like(out[kept]).requires_grad_()
+                kept_value = out[kept].clone()
+                loss = (w * out[kept]).sum()
+                out[written].mul_(2.0)
+                loss.backward()
+                assert torch.equal(w.grad, kept_value)
