@@ -115,10 +115,12 @@ def _f32(shape, dev: torch.device) -> torch.Tensor:
     return torch.empty(shape, device=dev, dtype=torch.float32)
 
 
-def _workspace(size: int, dev: torch.device) -> torch.Tensor:
-    """An allocation of its own, as every output has one: views of one buffer share a version counter, and writing to
-    one of them in place would invalidate a graph that has kept another."""
-    return torch.empty(size, device=dev, dtype=torch.uint8)
+def _buffers(workspace: int, dev: torch.device, *shapes):
+    """A workspace of `workspace` bytes (a multiple of 256) and float32 outputs of the given shapes.  Each is an
+    allocation of its own: views of one buffer share a version counter, and writing to one of them in place would
+    invalidate a graph that has kept another."""
+    ws = torch.empty(workspace >> 2, device=dev, dtype=torch.float32)
+    return (ws, *[ws.new_empty(s) for s in shapes])
 
 
 def _scalar_grad(holder: list, dloss: torch.Tensor) -> torch.Tensor:
@@ -170,7 +172,8 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, temperature: floa
     z = _rows(logits)
     y = _index(labels, logits.shape[:-1], logits.device, "labels")
     shape = y.shape
-    y = y.reshape(-1)
+    if len(shape) != 1:
+        y = y.reshape(-1)
     if _wants_grad(logits):
         logps = _TokenLogprobs.apply(z, y, float(temperature), int(ignore_index))
     else:
@@ -199,7 +202,7 @@ def _policy(z, y, old, adv, ref, w, clip_low, clip_high, kl_coef, entropy_coef, 
     n, V = z.shape
     dev = z.device
     size = 256 + (4 * n + 255) // 256 * 256  # kdn_policy_loss_workspace_size
-    ws, loss, logps, entropy = _workspace(size, dev), _f32((), dev), _f32(n, dev), _f32(n, dev)
+    ws, loss, logps, entropy = _buffers(size, dev, (), n, n)
     g = _grad_rows(z) if with_grad else None
     _call("kdn_policy_loss", dev, z.data_ptr(), _DTYPE[z.dtype], _ld(z), y.data_ptr(), _INDEX[y.dtype], ignore_index,
           old.data_ptr(), adv.data_ptr(), _lib.ptr(ref), _lib.ptr(w), clip_low, clip_high, kl_coef, entropy_coef,
@@ -280,7 +283,7 @@ def _preference(z, y, cu, ref, beta, label_smoothing, length_normalised, tempera
     dev = z.device
     pairs = (cu.numel() - 1) // 2
     size = 256 + sum((b + 255) // 256 * 256 for b in (8 * n, 4 * n, 4 * pairs))  # kdn_preference_loss_workspace_size
-    ws, loss, log_ratios, logps = _workspace(size, dev), _f32((), dev), _f32(2 * pairs, dev), _f32(n, dev)
+    ws, loss, log_ratios, logps = _buffers(size, dev, (), 2 * pairs, n)
     g = _grad_rows(z) if with_grad else None
     _call("kdn_preference_loss", dev, z.data_ptr(), _DTYPE[z.dtype], _ld(z), y.data_ptr(), _INDEX[y.dtype],
           ignore_index, cu.data_ptr(), pairs, _lib.ptr(ref), beta, label_smoothing, length_normalised, temperature,
@@ -349,7 +352,7 @@ def _distillation(z, t, ids, lse, w, temperature, with_grad):
     n, V = z.shape
     dev = z.device
     size = 256 + (4 * n + 255) // 256 * 256  # kdn_distillation_loss_workspace_size
-    ws, loss, divergence = _workspace(size, dev), _f32((), dev), _f32(n, dev)
+    ws, loss, divergence = _buffers(size, dev, (), n)
     g = _grad_rows(z) if with_grad else None
     _call("kdn_distillation_loss", dev, z.data_ptr(), _DTYPE[z.dtype], _ld(z), t.data_ptr(), _DTYPE[t.dtype],
           ids.data_ptr(), _INDEX[ids.dtype], t.shape[-1], _lib.ptr(lse), _lib.ptr(w), temperature, loss.data_ptr(),
