@@ -285,6 +285,11 @@ struct Cta {
 __device__ __forceinline__ float over_t(const LossRows& a, float x, float c) {
   return fmaf(x, a.inv_hi, fmaf(x, a.inv_lo, c));
 }
+// ... where x / T and c nearly cancel: what is rounded on the way is of the size of the result, not of c (whose unit in
+// the last place the product with the lower half is below)
+__device__ __forceinline__ float over_t_less(const LossRows& a, float x, float c) {
+  return fmaf(x, a.inv_lo, fmaf(x, a.inv_hi, c));
+}
 
 // Largest logit m of a part of a row, the sum s of exponentials below it and (kMoment) u = sum e^d d (base 2), which a
 // change of m shifts.
@@ -631,7 +636,7 @@ __device__ __forceinline__ float teacher_probabilities(const LossRows& a, const 
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if (id[i] < 0) continue;
-    lp[i] = t.lse ? over_t(a, lp[i], -lse) : over_t(a, lp[i] - m, -s);
+    lp[i] = t.lse ? over_t_less(a, lp[i], -lse) : over_t(a, lp[i] - m, -s);
     mass += expf(lp[i]);
   }
   mass = warp_sum(mass);
@@ -1567,7 +1572,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
       sum = logf(warp_sum(sum));
     }
     for (int k = lane; k < K; k += 32) {
-      const float lp = t.lse ? over_t(a, tp[k], -t.lse[r]) : over_t(a, tp[k] - tm, -sum);
+      const float lp = t.lse ? over_t_less(a, tp[k], -t.lse[r]) : over_t(a, tp[k] - tm, -sum);
       tp[k] = id[k] < 0 ? -INFINITY : lp;
       if (id[k] >= 0) ps += expf(lp);
     }

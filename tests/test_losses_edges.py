@@ -329,3 +329,36 @@ def test_outputs_of_a_call_are_tensors_of_their_own(grad):
                 out[written].mul_(2.0)
                 loss.backward()
                 assert torch.equal(w.grad, kept_value)
+
+
+# ------------------------------------------------------------------------------------------- the rest of the teacher
+@gpu
+@pytest.mark.parametrize("n,V,K,dtype", [(5, 700, 6, torch.float32), (40, 4099, 200, torch.bfloat16),
+                                         (300, 16411, 64, torch.bfloat16), (300, 8200, 20, torch.float32)])
+@pytest.mark.parametrize("T", [1.0, 0.7, 2.0])
+@pytest.mark.parametrize("offset", [0.0, 1000.0])
+def test_the_rest_of_the_teacher_is_as_exact_as_its_inputs(n, V, K, dtype, T, offset):
+    """t / T - lse of two numbers however large: its error is that of the difference.  With entries of |t / T - lse| below
+    16 for all but 2^-20 of the mass, each rounded twice (2^-21 each), an exponential of 2^-22 and a sum of up to 256, 1 - P
+    is within delta = 2^-19; log(p_r / q_r) multiplies it."""
+    import kdn_b200 as kdn
+
+    rng = np.random.default_rng(K)
+    z = _logits(n, V, dtype, seed=11, scale=0.5)
+    ids = np.stack([rng.permutation(V)[:K] for _ in range(n)])
+    t = (T * rng.standard_normal((n, K)) + offset).astype(np.float32)
+    lse = (np.logaddexp.reduce(t.astype(np.float64) / T, axis=1) - np.log(0.6 + 0.3 * rng.random(n))).astype(np.float32)
+    td, idd, ld = _cuda(t, ids, lse)
+    _, kl, d = kdn.distillation_loss_and_grad(z, td, idd, teacher_lse=ld, weights=torch.ones(n, device="cuda"),
+                                              temperature=T)
+    zz, got, g, delta = _np(z), _np(kl), _np(d), 2.0 ** -19
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    for r in range(0, n, max(1, n // 25)):
+        want, p, q, p_r, log_qr, out, rel = _rest_reference(zz[r], T, t[r].astype(np.float64), ids[r], float(lse[r]))
+        eps = 2.0 ** -23 * (zz[r].max() - zz[r].min()) / T + 2.0 ** -19
+        assert abs(got[r] - want) <= 2 * eps + delta * (abs(np.log(p_r) - log_qr) + 2)
+        ref = T * (q * (p.sum() + p_r) - p)
+        assert (np.abs(g[r][ids[r]] - ref) <= T * (2 * eps * q + 2 * delta * (p + q)) + np.abs(ref) * half).all()
+        ref = T * np.exp(rel[out]) * ((p.sum() + p_r) * np.exp(log_qr) - p_r)
+        size = T * np.exp(rel[out]) * ((p.sum() + p_r) * np.exp(log_qr) + p_r)
+        assert (np.abs(g[r][out] - ref) <= size * (2 * eps + 2 * delta / p_r) + np.abs(ref) * half + 1e-37).all()
