@@ -379,7 +379,8 @@ int kdn_varlen_causal_attention(const void* q, const void* k_cache, const void* 
  *     the ids' its logits lie (where all of them are -inf the divergence is +inf and the gradient outside the ids zero;
  *     where that mass is below 2^-126, a 1 - sum p below 2^-20 is rounding and counts as zero).
  *     divergence[t] = KL(p || q), loss = T^2 sum_t w_t divergence[t].
- *   kdn_scale_rows: x *= *scale in place (a device scalar); returns without touching x when it is 1.
+ *   kdn_scale_rows: x *= *scale in place (a device scalar), each product rounded to x's type; returns without touching x
+ *     when it is 1.
  * Workspaces: the *_workspace_size entries, 256-byte aligned.
  */
 int kdn_token_logprobs(const void* logits, int dtype, int64_t ld, const void* labels, int index_dtype,

@@ -668,8 +668,10 @@ __device__ __forceinline__ void add_at(float2* g, int e, float c) {
   }
 }
 
-// log2(e) / T in two halves: with one, its rounding moves every exponent of a row the same way, and the log of the
-// row's sum by as much as 1e-6.
+// log2(e) / T in two halves: with one, its rounding (up to 6e-8) moves every exponent of a part of a row the same way,
+// and the log of the row's sum by its distance from the part's largest logits, 1e-7 and more.  (A gradient's exponentials
+// and the few at the teacher's ids take the rounded factor: it moves a term at e^-7 by 4e-7 of itself, far below a bf16
+// gradient's rounding and a few units of the last place of an fp32 one.)
 struct Log2Scale {
   float hi, lo;
 };
@@ -1518,8 +1520,9 @@ __global__ void __launch_bounds__(Streaming<Terms>::kThreads, 1)
 // Teacher entries are held in shared memory; a bit per element of the share marks the teacher's ids, so that the
 // student's mass outside them is a sum of its own (one minus the mass inside would lose what is left when that is
 // near one).  The gradient is written densely, then the entries at the ids are written over.  For few rows, short rows
-// and more than 128 entries: 16 x 32000 bf16 with 32 entries 9 us, the latency of one row (teacher, statistics, merge,
-// gradient one after another); 4096 x 32000 with 64 entries 155 us, where the streaming kernel takes 124.
+// and more than 128 entries: 16 x 32000 bf16 with 32 entries 10 us with the sum of the losses, the latency of one row
+// (teacher, statistics, merge, gradient one after another).  4096 x 32000: 64 entries 175 us, where the streaming kernel
+// takes 118; 200 entries 259 us, with a rest class 206.
 template <typename T, int NT, bool kTail, bool kGrad>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, DistillTerms t, int parts) {
   extern __shared__ float sm[];
@@ -1528,7 +1531,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
   float* tp = sm;                                // [K] teacher logits, then probabilities
   int* id = reinterpret_cast<int*>(sm + K);      // [K] ids, -1 where there is none
   __shared__ uint32_t mark[NT * kNV / 4];        // a byte per vector of a round, a bit per element
-  __shared__ float ts[2];                        // sum of p; log of the teacher's sum of exponentials
+  __shared__ float mass;                         // the sum of p
   __shared__ int twice;                          // an id was given twice
   const int64_t r = blockIdx.x / unsigned(parts);
   const int rank = int(blockIdx.x % unsigned(parts));
@@ -1577,7 +1580,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
       if (id[k] >= 0) ps += expf(lp);
     }
     ps = warp_sum(ps);
-    if (lane == 0) ts[0] = ps;
+    if (lane == 0) mass = ps;
   }
   const int rounds = max(1, (w.v1 - w.v0 + NT * kNV - 1) / (NT * kNV));
   Apart st;  // without kTail: all of the row outside
@@ -1618,7 +1621,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_kernel(LossRows a, Dist
   }
   if (parts > 1) tc::cluster_wait();
   st = merge_rows<NT>(st, a, rank, parts);
-  const float ps = any ? ts[0] : -1.f;
+  const float ps = any ? mass : -1.f;
   const Rest rest = rest_of(a, kTail, ps, st);
   const float wt = t.weights ? t.weights[r] : t.scale ? *t.scale : mean_of_few(a, t.ids, K);
   if (rank == 0 && tid < 32) {
@@ -1798,7 +1801,9 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(LossRows a, PairTerm
 
 // x *= *scale; nothing is read or written where the scale is one, which is the common case (so the grid is small, and
 // its CTAs take share after share of a row: a warp 256 vectors, or 256 threads 2048).  One read, one write, bound by
-// memory: 8192 x 32000 bf16 in 165 us, 97 % of the measured copy rate.  A bf16 gradient is rounded a second time here.
+// memory: 8192 x 32000 bf16 in 165 us, 97 % of the measured copy rate.  A bf16 gradient is rounded a second time
+// here (the upstream gradient is not known when it is formed): within 2^-7 of itself instead of 2^-8 where the scale is no
+// power of two.
 template <typename T, int NT>
 __global__ void __launch_bounds__(kSmall) scale_kernel(LossRows a, const float* __restrict__ scale, int parts) {
   constexpr int kUnits = kSmall / NT;  // shares of a CTA

@@ -16,9 +16,15 @@ Logits are float32 or bfloat16, [..., vocab], with any row stride and alignment;
 weights and padding mean, and what -inf and NaN give stand at the entries of include/kdn.h.  Only logits receive a
 gradient, and in reverse mode alone: logits with a forward-mode tangent are refused.  The loss and its gradient come
 from one pass over the logits (two for ``preference_loss``), so ``loss.backward()`` only hands over what the forward
-formed (scaled by the upstream gradient where that is not one); the logits are not kept.  A second backward through one
-call raises.  ``*_loss_and_grad`` return the gradient directly, as a last value, for trainers that run their own head
-backward.  Losses, log-probabilities and statistics are float32.  Errors raise RuntimeError; there is no CPU path.
+formed (scaled by the upstream gradient where that is not one); the logits are not kept.  The gradient has the logits'
+type: a factor that is no power of two rounds a bf16 one a second time (put it into ``weights``, where it costs nothing).
+A second backward through one call raises.  ``*_loss_and_grad`` return the gradient directly, as a last value, for
+trainers that run their own head backward.  Losses, log-probabilities and statistics are float32.  Errors raise
+RuntimeError; there is no CPU path.
+
+Logits that no view makes [n, vocab] rows are copied: ``logits[:, :-1]`` of a [B, T, vocab] tensor is.  Pass all of them,
+with ignore_index as the label of the positions that predict nothing.  Logits whose first row starts off 16 bytes while
+their rows lie whole 16 bytes apart (``logits[:, 1:]`` of [n, vocab]) get a gradient of another 16-byte phase, stored element by element.
 """
 
 from __future__ import annotations
